@@ -17,6 +17,7 @@
 #ifndef SR_HIP_H
 #define SR_HIP_H
 
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -391,6 +392,73 @@ int sr_tecogan_set_vgg(sr_ctx* ctx, sr_vgg* v);
 #define SR_NOALLOC_SCRATCH_BYTES (32 * 1024 * 1024)
 int sr_op_conv3x3_wgrad_noalloc(int device, int dtype, int B, int H, int W, int Cin, int Cout, const float* d_x,
                                 const float* d_dy, float* d_dw, float* d_db, void* hip_stream);
+
+/* ---- operators of a residual trunk and of its training step on DEVICE tensors (no counterpart in the reference) --------------
+ * What a deeper trunk of residual blocks (reference layers.py:58-62) needs to stay trainable: norms before and after a block, and
+ * gradients clipped by their global norm.  All calls take DEVICE pointers, are asynchronous on `hip_stream` (a hipStream_t of
+ * `device`, NULL = its default stream), allocate nothing, keep nothing and can be captured into a HIP graph.  `device` need not be
+ * the caller's current device, which is restored on every path.  A workspace belongs to one call at a time: two calls that may
+ * overlap (on two streams, in two graphs) need one each.  Results do not depend on the run: no atomics, sums in a fixed order. */
+enum sr_type { SR_T_F32 = 0, SR_T_BF16 = 1, SR_T_F16 = 2 };          /* how a tensor is stored */
+enum sr_norm_kind { SR_NORM_RMS = 0, SR_NORM_LAYER = 1 };
+enum sr_norms { SR_NORM_POST = 1, SR_NORM_PRE = 2 };                 /* behind the block / before the next one; a bit mask */
+enum sr_gate_act { SR_GATE_LINEAR = 0, SR_GATE_SIGMOID = 1 };
+
+/* One residual block's output joined to the stream.  Row r of 1 <= `channels` <= 8192 values is one position (an NHWC pixel):
+ *   hat(v) = (v - m) / sqrt(mean((v - m)^2) + eps), m = mean(v) for SR_NORM_LAYER, 0 for SR_NORM_RMS
+ *   p = post_gain * hat(y) + post_bias   (norms without SR_NORM_POST: p = y)
+ *   h = x + scale * a * p                a = gate or sigmoid(gate), 1 without a gate
+ *   n = pre_gain * hat(h) + pre_bias     (norms with SR_NORM_PRE; the next block's input)
+ * `rows_per_gate` consecutive rows share a gate row (1: a gate value for every element; h * w: a channel gate for every image); it
+ * divides `rows` and is not looked at without a gate.  x, h, dx, dh have the stream's type; y, gate, n and their gradients the
+ * branch's, which is the stream's or, beside an fp32 stream, a 16-bit one; gains, biases and their gradients are dense fp32
+ * vectors, NULL = ones / zeros.  ld*: elements between rows (>= channels; the channels of a row are contiguous, any alignment of
+ * whole elements).  Sums and all values in between are fp32, with squares up to 3e38: |v| beyond 1e18 overflows them.
+ * sr_op_residual_norm: without a branch (y NULL: norms == SR_NORM_PRE, no gate) h is x and is not written.  h may be x or y, n may
+ *   be x or y (same type and pitch), gate too with rows_per_gate 1; otherwise outputs overlap nothing.
+ * sr_op_residual_norm_bwd: from h (needed with SR_NORM_PRE), y (with SR_NORM_POST or a gate), dh = the gradient that reaches h
+ *   through the stream (NULL: none; needed without SR_NORM_PRE) and dn (with SR_NORM_PRE) to dx = the whole gradient of h, dy (NULL:
+ *   there is no branch), dgate (NULL: not wanted) and the vectors that are not NULL.  Row statistics are taken again from h and y.
+ *   dx, dy may be h, y, dh or dn (same type and pitch).  rows == 0 zeroes the vectors.  `workspace`:
+ *   sr_op_residual_norm_bwd_workspace bytes (gate: whether there is one), 16-byte aligned. */
+typedef struct sr_residual_norm_desc {
+    int64_t rows, rows_per_gate;
+    int64_t ldx, ldy, ldg, ldh, ldn;             /* x, y, gate, h, n */
+    int64_t lddh, lddn, lddx, lddy, lddg;        /* dh, dn, dx, dy, dgate */
+    int32_t channels, stream_type, branch_type, kind, norms, gate_act;
+    float scale, eps;                            /* eps > 0 */
+} sr_residual_norm_desc;
+int sr_op_residual_norm(int device, const sr_residual_norm_desc* desc, const void* x, const void* y, const void* gate,
+                        const float* post_gain, const float* post_bias, const float* pre_gain, const float* pre_bias, void* h,
+                        void* n, void* hip_stream);
+int sr_op_residual_norm_bwd_workspace(const sr_residual_norm_desc* desc, int gate, size_t* bytes);
+int sr_op_residual_norm_bwd(int device, const sr_residual_norm_desc* desc, const void* h, const void* y, const void* gate,
+                            const float* post_gain, const float* post_bias, const float* pre_gain, const void* dh, const void* dn,
+                            void* dx, void* dy, void* dgate, float* dpost_gain, float* dpost_bias, float* dpre_gain, float* dpre_bias,
+                            void* workspace, size_t workspace_bytes, void* hip_stream);
+
+/* A list of dense tensors on one device (a model's gradients): `count` elements of enum sr_type `type` from `data` on, aligned to
+ * their elements; count may be 0.  The list holds addresses, not memory: it is valid as long as the tensors stay where they are, and
+ * may be used by several threads.  sr_tensors_workspace: bytes of workspace (8-byte aligned) the calls below need. */
+typedef struct sr_tensors sr_tensors;
+typedef struct sr_tensor_desc {
+    void* data;
+    int64_t count;
+    int32_t type;
+} sr_tensor_desc;
+int sr_tensors_create(sr_tensors** out, int device, int n, const sr_tensor_desc* tensors);
+int sr_tensors_destroy(sr_tensors* t);
+int sr_tensors_workspace(const sr_tensors* t, size_t* bytes);
+/* d_norm (one float) = scale * sqrt(sum of the squares of all elements), d_norms (nullable, one float a tensor) = the same of each
+ * tensor; scale > 0 (1 / ranks, 1 / loss scale).  Squares are added in 64 bits.  An infinity or NaN shows in the norm. */
+int sr_op_grad_norm(const sr_tensors* grads, float scale, float* d_norm, float* d_norms, void* workspace, size_t workspace_bytes,
+                    void* hip_stream);
+/* Gradient clipping as Keras 2.2.4's `clipnorm` does it (optimizers.py get_gradients / clip_norm): with norm as above, every element
+ * becomes g * scale * (max_norm / norm if norm > max_norm, else 1), rounded once to its type.  A NaN norm clips nothing, an
+ * infinite one leaves zeros (NaN where the infinity was), as the formula says; d_norm tells.  `out` (NULL: in place): a list
+ * of the same counts and types that is written instead; each of its tensors is the gradient itself or overlaps none. */
+int sr_op_clip_grads(const sr_tensors* grads, const sr_tensors* out, float max_norm, float scale, float* d_norm, void* workspace,
+                     size_t workspace_bytes, void* hip_stream);
 
 /* Measurement utility (no reference counterpart): times `iters` back-to-back launches
  * of one 3x3 conv (or stride-2 transposed conv) layer on device-resident random data

@@ -5,6 +5,7 @@ fallback: if the library or a HIP device is missing, calls raise.
 """
 from __future__ import annotations
 
+import collections
 import ctypes as C
 import os
 
@@ -110,6 +111,14 @@ SIGNATURES = {
     "sr_vgg_loss_grads": (C.c_int, [_vp, C.c_int, _vp, _vp, _f32p, _f32p, _vp]),
     "sr_tecogan_set_vgg": (C.c_int, [_vp, _vp]),
     "sr_op_conv3x3_wgrad_noalloc": (C.c_int, [C.c_int] * 7 + [_vp] * 5),
+    "sr_op_residual_norm": (C.c_int, [C.c_int] + [_vp] * 11),
+    "sr_op_residual_norm_bwd_workspace": (C.c_int, [_vp, C.c_int, C.POINTER(C.c_size_t)]),
+    "sr_op_residual_norm_bwd": (C.c_int, [C.c_int] + [_vp] * 17 + [C.c_size_t, _vp]),
+    "sr_tensors_create": (C.c_int, [C.POINTER(_vp), C.c_int, C.c_int, _vp]),
+    "sr_tensors_destroy": (C.c_int, [_vp]),
+    "sr_tensors_workspace": (C.c_int, [_vp, C.POINTER(C.c_size_t)]),
+    "sr_op_grad_norm": (C.c_int, [_vp, C.c_float, _vp, _vp, _vp, C.c_size_t, _vp]),
+    "sr_op_clip_grads": (C.c_int, [_vp, _vp, C.c_float, C.c_float, _vp, _vp, C.c_size_t, _vp]),
     "sr_bench_conv": (C.c_int, [C.c_int] * 10 + [C.POINTER(C.c_float)]),
 }
 
@@ -863,6 +872,278 @@ def conv3x3_wgrad_noalloc(B, H, W, Cin, Cout, d_x, d_dy, d_dw, d_db=None, dtype=
     """Device pointers (ints); asynchronous on `stream`.  Allocates nothing (include/sr_hip.h)."""
     _check(lib().sr_op_conv3x3_wgrad_noalloc(device, DTYPES[dtype], B, H, W, Cin, Cout, _vp(d_x), _vp(d_dy), _vp(d_dw),
                                              _vp(d_db) if d_db else None, _vp(stream) if stream else None))
+
+
+# ---------------------------------------------------------------- operators on device tensors (torch tensors on the GPU)
+_NORMS = {"post": 1, "pre": 2, "both": 3}
+_KINDS = {"rms": 0, "layer": 1}
+_GATES = {"linear": 0, "sigmoid": 1}
+_torch = None
+_torch_types = None
+
+
+class _ResidualNormDesc(C.Structure):
+    _fields_ = ([("rows", C.c_int64), ("rows_per_gate", C.c_int64)]
+                + [(n, C.c_int64) for n in ("ldx", "ldy", "ldg", "ldh", "ldn", "lddh", "lddn", "lddx", "lddy", "lddg")]
+                + [(n, C.c_int32) for n in ("channels", "stream_type", "branch_type", "kind", "norms", "gate_act")]
+                + [("scale", C.c_float), ("eps", C.c_float)])
+
+
+class _TensorDesc(C.Structure):
+    _fields_ = [("data", _vp), ("count", C.c_int64), ("type", C.c_int32)]
+
+
+def _types():
+    global _torch, _torch_types
+    if _torch_types is None:
+        import torch
+        _torch, _torch_types = torch, {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    return _torch_types
+
+
+def _type_of(t, what):
+    code = _types().get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what}: float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _stream_of(stream, device):
+    """The hipStream_t of a call: the caller's (an int), or torch's current stream of that device."""
+    return _torch.cuda.current_stream(device).cuda_stream if stream is None else int(stream)
+
+
+def _rows_of(t, what, C_, device, dtype=None, rows=None):
+    """Elements between the rows of t (..., C) seen as a matrix; the checks every tensor of a call goes through."""
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the call on {device}")
+    if t.dim() == 0 or t.shape[-1] != C_:
+        raise ValueError(f"{what}: expected {C_} channels in the last dimension, got shape {tuple(t.shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{what}: expected {dtype}, got {t.dtype}")
+    if rows is not None and t.numel() != rows * C_:
+        raise ValueError(f"{what}: expected {rows} rows of {C_}, got shape {tuple(t.shape)}")
+    if t.is_contiguous():
+        return C_
+    if C_ > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what}: the channels of a row must be contiguous")
+    try:
+        return t.view(-1, C_).stride(0)
+    except RuntimeError:
+        raise ValueError(f"{what}: the rows of shape {tuple(t.shape)} and strides {tuple(t.stride())} are not evenly spaced") from None
+
+
+def _vector(t, what, C_, device):
+    if t is None:
+        return None
+    if t.device != device or t.dtype != _torch.float32 or t.shape != (C_,) or not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous float32 vector of {C_} on {device}")
+    return t.data_ptr()
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _block(x, branch_dtype, gate, norms, kind, gate_act, scale, eps):
+    """(descriptor, rows, channels, device, pitch of the gate) of a residual-block call on x, the stream."""
+    if x.device.type != "cuda":
+        raise ValueError(f"the stream is on {x.device}: these operators have no CPU fallback")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"expected (..., channels), got shape {tuple(x.shape)}")
+    if norms not in _NORMS or kind not in _KINDS or gate_act not in _GATES:
+        raise ValueError(f"norms one of {sorted(_NORMS)}, kind one of {sorted(_KINDS)}, gate_act one of {sorted(_GATES)}")
+    C_ = x.shape[-1]
+    rows, rpg, ldg = x.numel() // C_, 1, 0
+    if gate is not None:
+        ldg = _rows_of(gate, "gate", C_, x.device, branch_dtype)
+        gates = gate.numel() // C_
+        if (rows % gates if gates else rows) != 0:
+            raise ValueError(f"gate: {gates} rows do not divide the {rows} rows of the stream")
+        rpg = rows // gates if gates and rows else 1
+    d = _ResidualNormDesc(rows=rows, rows_per_gate=rpg, ldg=ldg, channels=C_, stream_type=_type_of(x, "stream"),
+                          branch_type=_types()[branch_dtype], kind=_KINDS[kind], norms=_NORMS[norms], gate_act=_GATES[gate_act],
+                          scale=scale, eps=eps)
+    return d, rows, C_, x.device
+
+
+def residual_norm(x, y=None, gate=None, post_gain=None, post_bias=None, pre_gain=None, pre_bias=None, norms="both", kind="rms",
+                  gate_act="linear", scale=1.0, eps=1e-6, branch_dtype=None, h=None, n=None, stream=None):
+    """A residual block's output joined to its stream, with the norm behind the block and the one before the next
+    (include/sr_hip.h sr_op_residual_norm): h = x + scale * act(gate) * post(y), n = pre(h).  Torch tensors on one GPU, x (..., C)
+    the stream, y of the same shape the block's output; gate of the same shape, or (G, C) where G divides the rows: (B, C) gates
+    the channels of each image of an NHWC batch.  norms 'both', 'post' or 'pre', kind 'rms' or 'layer', gains and biases float32.
+    Without y: n = pre(x) in branch_dtype (default x's), and h is x.  h, n: tensors to write (h may be x, n may be y), default new
+    ones.  Returns (h, n), n None with norms 'post'.  Runs on `stream` (a hipStream_t as int), default torch's current one."""
+    tt = _types()
+    bt = y.dtype if y is not None else branch_dtype or x.dtype
+    if bt not in tt:
+        raise ValueError(f"y: float32, bfloat16 or float16, got {bt}")
+    if y is None and (norms != "pre" or gate is not None or h is not None):
+        raise ValueError("without y there is only norms='pre', and neither gate nor h")
+    d, rows, C_, dev = _block(x, bt, gate, norms, kind, gate_act, scale, eps)
+    d.ldx = _rows_of(x, "x", C_, dev)
+    if y is not None:
+        d.ldy = _rows_of(y, "y", C_, dev, bt, rows)
+        if h is None:
+            h = _torch.empty(x.shape, dtype=x.dtype, device=dev)
+        d.ldh = _rows_of(h, "h", C_, dev, x.dtype, rows)
+    if norms == "post":
+        if n is not None:
+            raise ValueError("norms='post' has no n")
+    else:
+        if n is None:
+            n = _torch.empty(x.shape, dtype=bt, device=dev)
+        d.ldn = _rows_of(n, "n", C_, dev, bt, rows)
+    _check(lib().sr_op_residual_norm(dev.index, C.byref(d), x.data_ptr(), _at(y), _at(gate), _vector(post_gain, "post_gain", C_, dev),
+                                     _vector(post_bias, "post_bias", C_, dev), _vector(pre_gain, "pre_gain", C_, dev),
+                                     _vector(pre_bias, "pre_bias", C_, dev), _at(h), _at(n), _stream_of(stream, dev)))
+    return (x if y is None else h), n
+
+
+ResidualNormGrads = collections.namedtuple("ResidualNormGrads", "dx dy dgate post_gain post_bias pre_gain pre_bias")
+
+
+def residual_norm_bwd(h, y=None, dh=None, dn=None, gate=None, post_gain=None, post_bias=None, pre_gain=None, norms="both",
+                      kind="rms", gate_act="linear", scale=1.0, eps=1e-6, bias_grads=False, branch=None, dx=None, dy=None,
+                      stream=None):
+    """Gradients of residual_norm (include/sr_hip.h sr_op_residual_norm_bwd) from its output h, the block's output y, the gradient
+    dh that reaches h through the stream (None: none) and dn, the gradient of n (with the pre norm).  -> ResidualNormGrads: dx, dy,
+    dgate (None without gate), and of the norms that are there the gains' and, with bias_grads, the biases' gradients (float32; of
+    every norm that is there, whether or not its gain is given).  branch False: the forward call had no y; then only dx and the
+    pre norm's vectors.  dx, dy: tensors to write, default new ones (dx may be dh, dy may be y or dn)."""
+    tt = _types()
+    post, pre = norms in ("post", "both"), norms in ("pre", "both")
+    if branch is None:
+        branch = post or y is not None
+    if (pre and dn is None) or (not pre and dh is None):
+        raise ValueError("dn is needed with the pre norm, dh without it")
+    if (post or gate is not None) and (y is None or not branch):
+        raise ValueError("y is needed with the post norm or a gate")
+    like = y if y is not None else dn if dn is not None else h
+    bt = like.dtype
+    if bt not in tt:
+        raise ValueError(f"y: float32, bfloat16 or float16, got {bt}")
+    d, rows, C_, dev = _block(h, bt, gate, norms, kind, gate_act, scale, eps)
+    d.ldh = _rows_of(h, "h", C_, dev)
+    if y is not None:
+        d.ldy = _rows_of(y, "y", C_, dev, bt, rows)
+    if dh is not None:
+        d.lddh = _rows_of(dh, "dh", C_, dev, h.dtype, rows)
+    if pre:
+        d.lddn = _rows_of(dn, "dn", C_, dev, bt, rows)
+    else:
+        dn = None
+    if dx is None:
+        dx = _torch.empty(h.shape, dtype=h.dtype, device=dev)
+    d.lddx = _rows_of(dx, "dx", C_, dev, h.dtype, rows)
+    if branch:
+        if dy is None:
+            dy = _torch.empty(h.shape, dtype=bt, device=dev)
+        d.lddy = _rows_of(dy, "dy", C_, dev, bt, rows)
+    elif dy is not None:
+        raise ValueError("dy without a branch")
+    dgate = None
+    if gate is not None:
+        dgate = _torch.empty(gate.shape, dtype=bt, device=dev)
+        d.lddg = C_
+    need = C.c_size_t()
+    _check(lib().sr_op_residual_norm_bwd_workspace(C.byref(d), int(gate is not None), C.byref(need)))
+    ws = _torch.empty(need.value, dtype=_torch.uint8, device=dev)
+    vec = _torch.empty((4, C_), dtype=_torch.float32, device=dev)
+    want = (post, post and bias_grads, pre, pre and bias_grads)
+    out = [vec[i] if w else None for i, w in enumerate(want)]
+    base = vec.data_ptr()
+    _check(lib().sr_op_residual_norm_bwd(dev.index, C.byref(d), h.data_ptr(), _at(y), _at(gate), _vector(post_gain, "post_gain", C_, dev),
+                                         _vector(post_bias, "post_bias", C_, dev), _vector(pre_gain, "pre_gain", C_, dev), _at(dh), _at(dn),
+                                         dx.data_ptr(), _at(dy), _at(dgate), *[base + 4 * C_ * i if w else None for i, w in enumerate(want)],
+                                         ws.data_ptr(), need.value, _stream_of(stream, dev)))
+    return ResidualNormGrads(dx, dy, dgate, *out)
+
+
+class TensorList:
+    """Dense torch tensors on one GPU -- a model's gradients -- as grad_norm and clip_grads take them (include/sr_hip.h
+    sr_tensors_create).  Any mix of float32, bfloat16 and float16, any sizes (0 too), any order of dimensions as long as the
+    elements leave no gaps.  Holds on to the tensors; a program whose gradients stay in the same buffers makes it once."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        _types()
+        self.device = self.tensors[0].device if self.tensors else _torch.device("cuda", _torch.cuda.current_device())
+        if self.device.type != "cuda":
+            raise ValueError(f"tensor 0 is on {self.device}: these operators have no CPU fallback")
+        desc = (_TensorDesc * max(len(self.tensors), 1))()
+        for i, t in enumerate(self.tensors):
+            if t.device != self.device:
+                raise ValueError(f"tensor {i} is on {t.device}, tensor 0 on {self.device}")
+            if not _dense(t):
+                raise ValueError(f"tensor {i} of shape {tuple(t.shape)} and strides {tuple(t.stride())} has gaps or repeats elements")
+            desc[i].data, desc[i].count, desc[i].type = t.data_ptr() or None, t.numel(), _type_of(t, f"tensor {i}")
+        self._h = _vp()
+        _check(lib().sr_tensors_create(C.byref(self._h), self.device.index, len(self.tensors), desc))
+        need = C.c_size_t()
+        _check(lib().sr_tensors_workspace(self._h, C.byref(need)))
+        self.workspace_bytes = need.value
+
+    def __len__(self):
+        return len(self.tensors)
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().sr_tensors_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _dense(t):
+    """Do the elements of t fill a stretch of memory exactly once?"""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def grad_norm(grads, scale=1.0, per_tensor=False, stream=None):
+    """Global L2 norm of many gradients (a TensorList or a sequence of tensors), times scale, as a float32 tensor (1,) on their GPU:
+    no synchronisation.  per_tensor: -> (norm, norms (n,)) with the norm of each.  include/sr_hip.h sr_op_grad_norm."""
+    if not isinstance(grads, TensorList):
+        grads = TensorList(grads)
+    if not grads._h:
+        raise ValueError("the TensorList is closed")
+    dev = grads.device
+    norm = _torch.empty(1, dtype=_torch.float32, device=dev)
+    each = _torch.empty(len(grads), dtype=_torch.float32, device=dev) if per_tensor else None
+    ws = _torch.empty(grads.workspace_bytes, dtype=_torch.uint8, device=dev)
+    _check(lib().sr_op_grad_norm(grads._h, scale, norm.data_ptr(), each.data_ptr() or None if per_tensor else None, ws.data_ptr(),
+                                 grads.workspace_bytes, _stream_of(stream, dev)))
+    return (norm, each) if per_tensor else norm
+
+
+def clip_grads(grads, max_norm, scale=1.0, out=None, stream=None):
+    """Scale gradients so that their global norm is at most max_norm (Keras' clipnorm): g * scale * min(1, max_norm / norm), in place
+    or into `out`, tensors of the same sizes and types.  grads, out: TensorLists or sequences of tensors.  Returns the norm before
+    clipping (of the gradients times scale) as a float32 tensor (1,), without a synchronisation.  include/sr_hip.h sr_op_clip_grads."""
+    if not isinstance(grads, TensorList):
+        grads = TensorList(grads)
+    if out is not None and not isinstance(out, TensorList):
+        out = TensorList(out)
+    if not grads._h or (out is not None and not out._h):
+        raise ValueError("the TensorList is closed")
+    dev = grads.device
+    norm = _torch.empty(1, dtype=_torch.float32, device=dev)
+    ws = _torch.empty(grads.workspace_bytes, dtype=_torch.uint8, device=dev)
+    _check(lib().sr_op_clip_grads(grads._h, out._h if out is not None else None, max_norm, scale, norm.data_ptr(), ws.data_ptr(),
+                                  grads.workspace_bytes, _stream_of(stream, dev)))
+    return norm
 
 
 def bench_conv(B, H, W, Cin, Cout, dtype="bf16x3", transposed=False, residual=False, iters=20, device=0):
