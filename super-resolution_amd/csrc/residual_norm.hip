@@ -12,10 +12,12 @@
 //   dpost_gain = sum dp hat(y), dpost_bias = sum dp, dpre_gain = sum dn hat(h), dpre_bias = sum dn
 //
 // Bound by HBM: the forward pass moves 4 tensors for ~16 operations an element, the backward pass 6 for ~40.  So a row is read
-// once: a group of lanes (a "team") holds it in registers, 8 elements a lane, across all sums of the row, and the backward pass
-// takes the row statistics again from what it holds instead of reading them.  Rows of up to 512 channels belong to 1..64 lanes of a
-// wave, several rows to a wave, and their sums are lane exchanges; longer rows belong to a workgroup, which joins its waves' sums
-// in LDS.  All sums and the values between them are fp32; tensors of 16 bits are rounded once, when they are stored.
+// once: a group of lanes (a "team") holds it in registers across all sums of the row, and the backward pass takes the row
+// statistics again from what it holds instead of reading them.  Rows of up to 512 channels belong to 1..64 lanes of a wave, several
+// rows to a wave, and their sums are lane exchanges; longer rows belong to a workgroup, which joins its waves' sums in LDS.  A lane
+// holds 8 elements of a row (4 in the backward pass of long rows, which otherwise spills: 8192 x 1000 takes 43 us instead of 50) and has
+// the same places of the team's next row on their way.  All sums and the values between them are fp32; tensors of 16 bits are rounded
+// once, when they are stored.
 #include "op_host.h"
 #include "row_math.h"
 
@@ -29,14 +31,24 @@ namespace {
 constexpr int MAX_C = 8192;          // 1024 lanes x 8 channels
 constexpr int WAVE_C = 512;          // up to here a row belongs to lanes of one wave
 
+enum Gate { G_NONE = 0, G_ROW = 1, G_SHARED = 2 };   // a gate row for every position / for several
+
+// Work split of a backward pass: `per_group` workgroups share the `span` rows of a group (the rows that share a gate row, or all
+// rows); that is a unit each.  Their teams take the group's rows in turn, so that what is read at one time lies together.
+struct Units {
+    unsigned span, units, per_group;
+};
+
+// what a call does, a bit each
+enum Flags { F_BRANCH = 1, F_POST = 2, F_PRE = 4, F_LAYER = 8, F_SIGMOID = 16, F_STREAM_GRAD = 32, F_READ_Y = 64 };
+
 struct FwdArgs {
     const void *x, *y, *gate;
     const float *pw, *pb, *qw, *qb;  // post gain / bias, pre gain / bias
     void *h, *n;
-    int64_t ldx, ldy, ldg, ldh, ldn;
-    unsigned rows, rpg;              // rpg: rows that share a gate row
-    int C, tl;                       // tl: log2 of a team's lanes (rows within a wave)
-    int layer, post, pre, sigmoid;
+    int ldx, ldy, ldg, ldh, ldn;
+    unsigned rows, span;             // span: rows that share a gate row
+    int C, tl, flags;                // tl: log2 of a team's lanes (rows within a wave)
     float scale, eps, inv_c;
 };
 
@@ -46,25 +58,30 @@ struct BwdArgs {
     void *dx, *dy, *dgate;
     float *part;                     // [blocks][nslot][C] partial sums of the gains' and biases' gradients
     float *gpart;                    // [units][C] partial sums of dgate where a gate row spans several units
-    int64_t ldh, ldy, ldg, lddh, lddn, lddx, lddy, lddg;
-    unsigned span;                   // rows of a group: those that share a gate row, or all
-    unsigned units, chunk, per_group;   // a unit is `chunk` rows of one group; per_group units make up a group
-    int by_row;                      // the gate has a row for every position
-    int C, tl;
-    int layer, post, pre, sigmoid;
+    int ldh, ldy, ldg, lddh, lddn, lddx, lddy, lddg;
+    Units u;
+    int C, tl, flags;
     int nslot, slot[4];              // where post gain, post bias, pre gain, pre bias are in `part`; -1: not wanted
     float scale, eps, inv_c;
 };
 
-// What a thread knows about its place in a team.  A lane holds 8 elements as 8 / VEC vectors, `team` vectors apart.
-template <int VEC, bool BLK>
+template <typename T>
+__device__ __forceinline__ T* row_of(const void* p, unsigned r, int ld) {
+    return (T*)p + (int64_t)((uint64_t)r * (unsigned)ld);
+}
+
+// What a thread knows about its place in a team.  A lane holds E elements as NV = E / VEC vectors, `lanes` vectors apart.
+// TAIL: the row's last vector is not full (`part` elements of it are).
+template <int E_, int VEC_, bool BLK_, bool TAIL_>
 struct Team {
+    static constexpr int E = E_, VEC = VEC_, NV = E / VEC;
+    static constexpr bool BLK = BLK_, TAIL = TAIL_;
     int lanes, lane, row, rows;      // lanes of a team, this thread's lane, its team's number in the workgroup, teams in the workgroup
-    int tl, C;
-    float* red;                      // BLK: [2][16][8] floats
+    int tl, C, part;
+    float* red;                      // BLK: [2][16][E] floats
     int phase = 0;
 
-    __device__ Team(int tl_, int C_, float* red_) : tl(tl_), C(C_), red(red_) {
+    __device__ Team(int tl_, int C_, float* red_) : tl(tl_), C(C_), part(C_ % VEC), red(red_) {
         if (BLK) {
             lanes = blockDim.x, lane = threadIdx.x, row = 0, rows = 1;
         } else {
@@ -72,6 +89,18 @@ struct Team {
         }
     }
     __device__ __forceinline__ int col(int j) const { return (j * lanes + lane) * VEC; }
+    __device__ __forceinline__ bool full(int j) const { return col(j) + VEC <= C; }
+    // does vector j hold the end of a row, and not all of it the row's?
+    __device__ __forceinline__ bool ends(int j) const { return TAIL && !full(j) && col(j) < C; }
+    // the place of column c in its vector
+    __device__ __forceinline__ int place(int c) const {
+        int d = c - (C - part);
+        if (!TAIL || d < 0) return c % VEC;
+        const int n4 = VEC == 8 ? part & 4 : 0;
+        if (d < n4) return d;
+        d -= n4;
+        return d < (part & 2) ? VEC - 4 + d : VEC - 2;
+    }
 
     // sums of K values over the team, in every lane
     template <int K>
@@ -95,262 +124,470 @@ struct Team {
     }
 };
 
-template <typename T, int VEC, bool TAIL, bool BLK>
-__device__ __forceinline__ void load_row(const T* p, const Team<VEC, BLK>& t, float (&v)[8]) {
+// A lane's elements of a row as they are stored.  Lanes behind the row never load: what they hold stays 0 from here on, so the
+// loads of a row are one branch and no selects.  A last vector of `part` < VEC elements is loaded and stored in pieces of 4, 2 and
+// 1, which have fixed places in the vector: the order of a row's elements in registers does not matter.
+template <typename T, typename TEAM>
+struct Raw {
+    Vec<T, TEAM::VEC> v[TEAM::NV];
+    T one;                           // the piece of 1
+    __device__ Raw() {
 #pragma unroll
-    for (int j = 0; j < 8 / VEC; ++j) {
-        const int c = t.col(j);
-        float o[VEC];
-        if (c + VEC <= t.C) {
-            load_vec<T, VEC>(p + c, o);
-        } else {
+        for (int j = 0; j < TEAM::NV; ++j)
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) o[k] = TAIL && c + k < t.C ? (float)p[c + k] : 0.f;
-        }
+            for (int k = 0; k < TEAM::VEC; ++k) v[j].v[k] = (T)0.f;
+        one = (T)0.f;
+    }
+};
+
+template <typename T, typename TEAM>
+__device__ __forceinline__ void load_raw(const T* p, int j, const TEAM& t, Raw<T, TEAM>& o) {
+    o.v[j] = *reinterpret_cast<const Vec<T, TEAM::VEC>*>(p + t.col(j));
+}
+
+template <typename T, typename TEAM>
+__device__ __forceinline__ void load_part(const T* p, int j, const TEAM& t, Raw<T, TEAM>& o) {
+    constexpr int VEC = TEAM::VEC;
+    const T* q = p + t.col(j);
+    if (VEC == 8 && (t.part & 4)) {
+        const Vec<T, 4> a = *reinterpret_cast<const Vec<T, 4>*>(q);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) v[j * VEC + k] = o[k];
+        for (int k = 0; k < 4; ++k) o.v[j].v[k] = a.v[k];
+    }
+    if (t.part & 2) {
+        const Vec<T, 2> a = *reinterpret_cast<const Vec<T, 2>*>(q + (t.part & 4));
+        o.v[j].v[VEC - 4] = a.v[0], o.v[j].v[VEC - 3] = a.v[1];
+    }
+    if (t.part & 1) o.one = q[t.part & 6];
+}
+
+template <typename T, typename TEAM>
+__device__ __forceinline__ void unpack(const Raw<T, TEAM>& r, const TEAM& t, float (&v)[TEAM::E]) {
+    constexpr int VEC = TEAM::VEC;
+#pragma unroll
+    for (int j = 0; j < TEAM::NV; ++j) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[j * VEC + k] = (float)r.v[j].v[k];
+        if (TEAM::TAIL && t.ends(j)) v[j * VEC + VEC - 2] = (float)r.one;
     }
 }
 
-template <typename T, int VEC, bool TAIL, bool BLK>
-__device__ __forceinline__ void store_row(T* p, const Team<VEC, BLK>& t, const float (&v)[8]) {
+// zeros in the places of a last vector that are not the row's
+template <typename TEAM>
+__device__ __forceinline__ void trim(float (&v)[TEAM::E], const TEAM& t) {
+    constexpr int VEC = TEAM::VEC;
+    if (!TEAM::TAIL) return;
 #pragma unroll
-    for (int j = 0; j < 8 / VEC; ++j) {
-        const int c = t.col(j);
+    for (int j = 0; j < TEAM::NV; ++j) {
+        if (!t.ends(j)) continue;
+        if (VEC == 8 && !(t.part & 4)) v[j * VEC] = v[j * VEC + 1] = v[j * VEC + 2] = v[j * VEC + 3] = 0.f;
+        if (!(t.part & 2)) v[j * VEC + VEC - 4] = v[j * VEC + VEC - 3] = 0.f;
+        if (!(t.part & 1)) v[j * VEC + VEC - 2] = 0.f;
+        v[j * VEC + VEC - 1] = 0.f;
+    }
+}
+
+template <typename T, typename TEAM>
+__device__ __forceinline__ void store_row(T* p, const TEAM& t, const float (&v)[TEAM::E]) {
+    constexpr int VEC = TEAM::VEC;
+#pragma unroll
+    for (int j = 0; j < TEAM::NV; ++j) {
         float o[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) o[k] = v[j * VEC + k];
-        if (c + VEC <= t.C) {
-            store_vec<T, VEC>(p + c, o);
-        } else if (TAIL) {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k)
-                if (c + k < t.C) p[c + k] = (T)o[k];
+        T* q = p + t.col(j);
+        if (t.full(j)) {
+            store_vec<T, VEC>(q, o);
+        } else if (TEAM::TAIL && t.col(j) < t.C) {
+            if (VEC == 8 && (t.part & 4)) {
+                const float w[4] = {o[0], o[1], o[2], o[3]};
+                store_vec<T, 4>(q, w);
+            }
+            if (t.part & 2) {
+                const float w[2] = {o[VEC - 4], o[VEC - 3]};
+                store_vec<T, 2>(q + (t.part & 4), w);
+            }
+            if (t.part & 1) q[t.part & 6] = (T)o[VEC - 2];
         }
     }
 }
 
-// v -= mean over the row (0 beyond it)
-template <int VEC, bool TAIL, bool BLK>
-__device__ __forceinline__ void centre(float (&v)[8], float mean, const Team<VEC, BLK>& t) {
+// v -= mean over the row; v is 0 behind it and stays so
+template <typename TEAM>
+__device__ __forceinline__ void centre(float (&v)[TEAM::E], float mean, const TEAM& t) {
 #pragma unroll
-    for (int j = 0; j < 8 / VEC; ++j)
+    for (int j = 0; j < TEAM::NV; ++j) {
+        const float m = t.col(j) < t.C ? mean : 0.f;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) v[j * VEC + k] = t.col(j) + k < t.C ? v[j * VEC + k] - mean : 0.f;
+        for (int k = 0; k < TEAM::VEC; ++k) v[j * TEAM::VEC + k] -= m;
+    }
+    trim(v, t);
 }
 
-__device__ __forceinline__ float sum8(const float (&v)[8]) {
-    return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-}
-__device__ __forceinline__ float dot8(const float (&a)[8], const float (&b)[8]) {
+template <int E>
+__device__ __forceinline__ float sum_e(const float (&v)[E]) {
     float s = 0.f, u = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; k += 2) s += a[k] * b[k], u += a[k + 1] * b[k + 1];
+    for (int k = 0; k < E; k += 2) s += v[k], u += v[k + 1];
+    return s + u;
+}
+template <int E>
+__device__ __forceinline__ float dot_e(const float (&a)[E], const float (&b)[E]) {
+    float s = 0.f, u = 0.f;
+#pragma unroll
+    for (int k = 0; k < E; k += 2) s += a[k] * b[k], u += a[k + 1] * b[k + 1];
     return s + u;
 }
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + expf(-g)); }   // rcp: 1 ulp
 
-template <int VEC, bool TAIL, bool BLK>
-__device__ __forceinline__ void load_gain(const float* p, const Team<VEC, BLK>& t, float (&v)[8], float none) {
+// one row of anything, 0 behind it
+template <typename T, typename TEAM>
+__device__ __forceinline__ void load_row(const T* p, const TEAM& t, float (&v)[TEAM::E]) {
+    Raw<T, TEAM> r;
+#pragma unroll
+    for (int j = 0; j < TEAM::NV; ++j) {
+        if (t.full(j)) load_raw(p, j, t, r);
+        else if (t.ends(j)) load_part(p, j, t, r);
+    }
+    unpack(r, t, v);
+}
+
+// a gain or bias, `none` where there is no vector; 0 behind the row, so that what is multiplied by it needs no mask
+template <typename TEAM>
+__device__ __forceinline__ void load_gain(const float* p, const TEAM& t, float (&v)[TEAM::E], float none) {
     if (p) {
-        load_row<float, VEC, TAIL, BLK>(p, t, v);
-    } else {                         // 0 beyond the row: what is multiplied by a gain needs no further mask
+        load_row(p, t, v);
+    } else {
 #pragma unroll
-        for (int j = 0; j < 8 / VEC; ++j)
+        for (int j = 0; j < TEAM::NV; ++j)
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) v[j * VEC + k] = t.col(j) + k < t.C ? none : 0.f;
+            for (int k = 0; k < TEAM::VEC; ++k) v[j * TEAM::VEC + k] = t.col(j) < t.C ? none : 0.f;
+        trim(v, t);
     }
 }
 
 // ------------------------------------------------------------------------------------------------- forward
-// v becomes hat(v); returns nothing else, the statistics live only here
-template <int VEC, bool TAIL, bool BLK>
-__device__ __forceinline__ void normalise(float (&v)[8], const FwdArgs& a, Team<VEC, BLK>& t) {
-    if (a.layer) {
-        float m[1] = {sum8(v)};
+template <typename TEAM>
+__device__ __forceinline__ void normalise(float (&v)[TEAM::E], const FwdArgs& a, TEAM& t) {
+    if (a.flags & F_LAYER) {
+        float m[1] = {sum_e(v)};
         t.sum(m);
-        centre<VEC, TAIL, BLK>(v, m[0] * a.inv_c, t);
+        centre(v, m[0] * a.inv_c, t);
     }
-    float s[1] = {dot8(v, v)};
+    float s[1] = {dot_e(v, v)};
     t.sum(s);
     const float rs = rsqrtf(s[0] * a.inv_c + a.eps);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] *= rs;
+    for (int k = 0; k < TEAM::E; ++k) v[k] *= rs;
 }
 
-template <typename TS, typename TB, int VEC, bool TAIL, bool BLK>
+// The teams of all workgroups take the rows in turn, so that what is read at one time lies together: with a stretch of rows for each
+// workgroup instead, the 942,080 x 64 call took 195 us instead of 139.
+template <typename TS, typename TB, int E, int VEC, bool BLK, bool TAIL, int GATE>
 __global__ void __launch_bounds__(BLK ? 1024 : 256) rn_fwd_kernel(const FwdArgs a) {
+    using TEAM = Team<E, VEC, BLK, TAIL>;
     __shared__ float red[BLK ? 256 : 1];
-    Team<VEC, BLK> t(a.tl, a.C, red);
-    float pw[8], pb[8], qw[8], qb[8];
-    load_gain<VEC, TAIL, BLK>(a.pw, t, pw, 1.f);
-    load_gain<VEC, TAIL, BLK>(a.pb, t, pb, 0.f);
-    load_gain<VEC, TAIL, BLK>(a.qw, t, qw, 1.f);
-    load_gain<VEC, TAIL, BLK>(a.qb, t, qb, 0.f);
-    for (unsigned r = blockIdx.x * t.rows + t.row; r < a.rows; r += gridDim.x * t.rows) {
-        float h[8], p[8], g[8];
-        load_row<TS, VEC, TAIL, BLK>((const TS*)a.x + r * a.ldx, t, h);
-        if (a.y) {
-            load_row<TB, VEC, TAIL, BLK>((const TB*)a.y + r * a.ldy, t, p);
-            if (a.gate) load_row<TB, VEC, TAIL, BLK>((const TB*)a.gate + (a.rpg == 1 ? r : r / a.rpg) * a.ldg, t, g);
-            if (a.post) {
-                normalise<VEC, TAIL, BLK>(p, a, t);
+    TEAM t(a.tl, a.C, red);
+    float pw[E], pb[E], qw[E], qb[E];
+    Raw<TS, TEAM> x;
+    Raw<TB, TEAM> y, g;
+    auto fetch = [&](unsigned r) {
+        const TS* px = row_of<const TS>(a.x, r, a.ldx);
+        const TB *py = row_of<const TB>(a.y, r, a.ldy), *pg = row_of<const TB>(a.gate, r, a.ldg);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) p[k] = p[k] * pw[k] + pb[k];
+        for (int j = 0; j < TEAM::NV; ++j) {
+            if (t.full(j)) {
+                load_raw(px, j, t, x);
+                if (a.flags & F_BRANCH) load_raw(py, j, t, y);
+                if (GATE == G_ROW) load_raw(pg, j, t, g);
+            } else if (t.ends(j)) {
+                load_part(px, j, t, x);
+                if (a.flags & F_BRANCH) load_part(py, j, t, y);
+                if (GATE == G_ROW) load_part(pg, j, t, g);
             }
-            if (a.gate) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) p[k] *= a.sigmoid ? sigmoid(g[k]) : g[k];
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) h[k] += a.scale * p[k];
-            store_row<TS, VEC, TAIL, BLK>((TS*)a.h + r * a.ldh, t, h);
         }
-        if (a.pre) {
-            normalise<VEC, TAIL, BLK>(h, a, t);
+    };
+    unsigned r = blockIdx.x * t.rows + t.row;
+    const unsigned step = gridDim.x * t.rows;
+    if (r < a.rows) fetch(r);
+    load_gain(a.pw, t, pw, 1.f);
+    load_gain(a.pb, t, pb, 0.f);
+    load_gain(a.qw, t, qw, 1.f);
+    load_gain(a.qb, t, qb, 0.f);
+    float act[E];                    // scale times the gate that rows share, and the first row behind them
+    unsigned end = 0;
+    for (; r < a.rows; r += step) {
+        float h[E], p[E], gt[E];
+        unpack(x, t, h);
+        unpack(y, t, p);
+        if (GATE == G_ROW) unpack(g, t, gt);
+        // the team's next row is on its way while this one is worked on
+        if (r + step < a.rows) fetch(r + step);
+        if (GATE == G_SHARED && r >= end) {
+            const unsigned group = r / a.span;
+            end = (group + 1) * a.span;
+            load_row(row_of<const TB>(a.gate, group, a.ldg), t, act);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) h[k] = h[k] * qw[k] + qb[k];
-            store_row<TB, VEC, TAIL, BLK>((TB*)a.n + r * a.ldn, t, h);
+            for (int k = 0; k < E; ++k) act[k] = a.scale * (a.flags & F_SIGMOID ? sigmoid(act[k]) : act[k]);
+        }
+        if (a.flags & F_BRANCH) {
+            if (a.flags & F_POST) {
+                normalise(p, a, t);
+#pragma unroll
+                for (int k = 0; k < E; ++k) p[k] = p[k] * pw[k] + pb[k];
+            }
+            if (GATE == G_ROW) {
+#pragma unroll
+                for (int k = 0; k < E; ++k) p[k] *= a.flags & F_SIGMOID ? sigmoid(gt[k]) : gt[k];
+            }
+#pragma unroll
+            for (int k = 0; k < E; ++k) h[k] += (GATE == G_SHARED ? act[k] : a.scale) * p[k];
+            store_row(row_of<TS>(a.h, r, a.ldh), t, h);
+        }
+        if (a.flags & F_PRE) {
+            normalise(h, a, t);
+#pragma unroll
+            for (int k = 0; k < E; ++k) h[k] = h[k] * qw[k] + qb[k];
+            store_row(row_of<TB>(a.n, r, a.ldn), t, h);
         }
     }
 }
 
 // ------------------------------------------------------------------------------------------------- backward
-// Sums of an accumulator over the teams of a workgroup; the threads of team 0 end with them.  `buf`: 4 waves x 512 floats.
-template <int VEC>
-__device__ __forceinline__ void join_teams(float (&v)[8], const Team<VEC, false>& t, float* buf) {
+// The sums over rows that a thread keeps for its 8 columns, in LDS: in registers the four of them would cost a wave in four, and
+// LDS has the time (two 16-byte reads and writes a sum and row, under a tenth of what the row takes to arrive).
+// [sum][half][thread] float4: no bank conflicts, and each thread's are its own until they are joined.
+template <int E>
+struct Sums {
+    static constexpr int Q = E / 4;
+    float4* at;
+    int step;
+    __device__ Sums(float* lds, int threads) : at(reinterpret_cast<float4*>(lds) + threadIdx.x), step(threads) {}
+    __device__ __forceinline__ void zero(int i) const {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-        for (int d = t.lanes; d < 64; d <<= 1) v[k] += __shfl_xor(v[k], d);
-    const int wave = threadIdx.x >> 6;
-    __syncthreads();                 // the buffer's last readers are done
-    if ((threadIdx.x & 63) < t.lanes) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) buf[wave * 512 + k * 64 + t.lane] = v[k];
+        for (int q = 0; q < Q; ++q) at[(Q * i + q) * step] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    __syncthreads();
-    if ((int)threadIdx.x < t.lanes) {
+    __device__ __forceinline__ void add(int i, const float (&v)[E]) const {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = (buf[k * 64 + t.lane] + buf[512 + k * 64 + t.lane]) + (buf[1024 + k * 64 + t.lane] + buf[1536 + k * 64 + t.lane]);
+        for (int q = 0; q < Q; ++q) {
+            float4 a = at[(Q * i + q) * step];
+            a.x += v[4 * q], a.y += v[4 * q + 1], a.z += v[4 * q + 2], a.w += v[4 * q + 3];
+            at[(Q * i + q) * step] = a;
+        }
+    }
+    __device__ __forceinline__ void get(int i, float (&v)[E]) const {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const float4 a = at[(Q * i + q) * step];
+            v[4 * q] = a.x, v[4 * q + 1] = a.y, v[4 * q + 2] = a.z, v[4 * q + 3] = a.w;
+        }
+    }
+    __device__ __forceinline__ void set(int i, const float (&v)[E]) const {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) at[(Q * i + q) * step] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    }
+};
+
+// Column c of sum i over the teams of a workgroup of four waves
+template <typename TEAM>
+__device__ __forceinline__ float joined(int i, int c, const TEAM& t, const float* lds) {
+    // element e of thread l of every team
+    const int l = c / TEAM::VEC % t.lanes, e = c / TEAM::VEC / t.lanes * TEAM::VEC + t.place(c);
+    const float* p = lds + ((Sums<TEAM::E>::Q * i + e / 4) * 256 + l) * 4 + e % 4;
+    float s = 0.f;
+#pragma unroll 8
+    for (int q = 0; q < t.rows; ++q) s += p[q * t.lanes * 4];
+    return s;
+}
+
+// Sum i over the teams of a workgroup to out[0 .. C), on top of what is there with `add`; the same thread has the same column
+// every time
+template <typename T, typename TEAM>
+__device__ __forceinline__ void leave(int i, const Sums<TEAM::E>& sums, const TEAM& t, const float* lds, T* out, bool add) {
+    if constexpr (TEAM::BLK) {
+        float v[TEAM::E], o[TEAM::E];
+        sums.get(i, v);
+        if (add) {
+            load_row(out, t, o);
+#pragma unroll
+            for (int k = 0; k < TEAM::E; ++k) v[k] += o[k];
+        }
+        store_row(out, t, v);
+    } else {
+        for (int c = threadIdx.x; c < t.C; c += 256) {
+            const float s = joined(i, c, t, lds);
+            out[c] = (T)(add ? (float)out[c] + s : s);
+        }
     }
 }
 
-template <typename TS, typename TB, int VEC, bool TAIL, bool BLK>
-__global__ void __launch_bounds__(BLK ? 1024 : 256) rn_bwd_kernel(const BwdArgs a) {
-    __shared__ float buf[BLK ? 256 : 2048];
-    Team<VEC, BLK> t(a.tl, a.C, buf);
-    float pw[8], pb[8], qw[8];
-    load_gain<VEC, TAIL, BLK>(a.pw, t, pw, 1.f);
-    load_gain<VEC, TAIL, BLK>(a.pb, t, pb, 0.f);
-    load_gain<VEC, TAIL, BLK>(a.qw, t, qw, 1.f);
-    float s_pw[8] = {}, s_pb[8] = {}, s_qw[8] = {}, s_qb[8] = {};
-    const bool shared_gate = a.dgate && !a.by_row;
-    for (unsigned u = blockIdx.x; u < a.units; u += gridDim.x) {
-        const unsigned group = u / a.per_group, first = (u - group * a.per_group) * a.chunk;
-        const unsigned r0 = group * a.span + first, r1 = r0 + min(a.chunk, a.span - first);
-        float s_g[8] = {};
-        for (unsigned r = r0 + t.row; r < r1; r += t.rows) {
-            float hv[8], yv[8], T[8], g[8], gt[8];
-            if (a.pre) load_row<TS, VEC, TAIL, BLK>((const TS*)a.h + r * a.ldh, t, hv);
-            if (a.y) load_row<TB, VEC, TAIL, BLK>((const TB*)a.y + r * a.ldy, t, yv);
-            if (a.pre) load_row<TB, VEC, TAIL, BLK>((const TB*)a.dn + r * a.lddn, t, g);
-            if (a.dh) {
-                load_row<TS, VEC, TAIL, BLK>((const TS*)a.dh + r * a.lddh, t, T);
-            } else {
+// FULL: layer norms or gradients of biases; without, only what rms norms with gains need is in registers.  The sums over rows are
+// those of a unit; a workgroup with several units adds them up in its partial sums.  With a gate that a unit shares they are
+//   A = sum T hat(y) (or T y), B = sum T   (T with the scale):  dpost_gain = a A, dpost_bias = a B, dgate = a' (post_gain A + post_bias B)
+template <typename TS, typename TB, int E, int VEC, bool BLK, bool TAIL, int GATE, bool FULL>
+__global__ void __launch_bounds__(BLK ? 1024 : 256, BLK ? 4 : 3) rn_bwd_kernel(const BwdArgs a) {
+    extern __shared__ float lds[];   // the sums, then BLK's [2][16][E] floats
+    enum { S_PW, S_QW, S_PB, S_QB };
+    using TEAM = Team<E, VEC, BLK, TAIL>;
+    TEAM t(a.tl, a.C, lds + (FULL ? 4 : GATE == G_SHARED ? 3 : 2) * E * blockDim.x);
+    const Sums<E> sums(lds, BLK ? blockDim.x : 256);
+    constexpr bool SUM_T = FULL || GATE == G_SHARED;
+    float pw[E], qw[E];
+    Raw<TS, TEAM> hr, dr;
+    Raw<TB, TEAM> yr, nr, gr;
+    auto fetch = [&](unsigned r) {
+        const TS *ph = row_of<const TS>(a.h, r, a.ldh), *pd = row_of<const TS>(a.dh, r, a.lddh);
+        const TB *py = row_of<const TB>(a.y, r, a.ldy), *pn = row_of<const TB>(a.dn, r, a.lddn), *pg = row_of<const TB>(a.gate, r, a.ldg);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) T[k] = 0.f;
+        for (int j = 0; j < TEAM::NV; ++j) {
+            if (t.full(j)) {
+                if (a.flags & F_PRE) load_raw(ph, j, t, hr), load_raw(pn, j, t, nr);
+                if (a.flags & F_READ_Y) load_raw(py, j, t, yr);
+                if (a.flags & F_STREAM_GRAD) load_raw(pd, j, t, dr);
+                if (GATE == G_ROW) load_raw(pg, j, t, gr);
+            } else if (t.ends(j)) {
+                if (a.flags & F_PRE) load_part(ph, j, t, hr), load_part(pn, j, t, nr);
+                if (a.flags & F_READ_Y) load_part(py, j, t, yr);
+                if (a.flags & F_STREAM_GRAD) load_part(pd, j, t, dr);
+                if (GATE == G_ROW) load_part(pg, j, t, gr);
             }
-            if (a.gate) load_row<TB, VEC, TAIL, BLK>((const TB*)a.gate + (a.by_row ? r : group) * a.ldg, t, gt);
-            if (a.layer) {
-                float m[2] = {a.pre ? sum8(hv) : 0.f, a.post ? sum8(yv) : 0.f};
+        }
+    };
+    for (unsigned u = blockIdx.x; u < a.u.units; u += gridDim.x) {
+        const unsigned group = u / a.u.per_group, r1 = (group + 1) * a.u.span, step = a.u.per_group * t.rows;
+        const unsigned r0 = group * a.u.span + (u - group * a.u.per_group) * t.rows + t.row;
+        if (r0 < r1) fetch(r0);
+        if (u == blockIdx.x) {
+            load_gain(a.pw, t, pw, 1.f);
+            load_gain(a.qw, t, qw, 1.f);
+        }
+        sums.zero(S_PW), sums.zero(S_QW);
+        if (SUM_T) sums.zero(S_PB);
+        if (FULL) sums.zero(S_QB);
+        float act[E];
+        if (GATE == G_SHARED) {
+            load_row(row_of<const TB>(a.gate, group, a.ldg), t, act);
+#pragma unroll
+            for (int k = 0; k < E; ++k) act[k] = a.flags & F_SIGMOID ? sigmoid(act[k]) : act[k];
+        }
+        for (unsigned r = r0; r < r1; r += step) {
+            float hv[E], yv[E], T[E], g[E], gt[E];
+            unpack(hr, t, hv);
+            unpack(nr, t, g);
+            unpack(yr, t, yv);
+            unpack(dr, t, T);
+            if (GATE == G_ROW) unpack(gr, t, gt);
+            if (r + step < r1) fetch(r + step);
+            float s[FULL ? 4 : 3];
+            if (FULL && (a.flags & F_LAYER)) {
+                float m[2] = {sum_e(hv), sum_e(yv)};
                 t.sum(m);
-                if (a.pre) centre<VEC, TAIL, BLK>(hv, m[0] * a.inv_c, t);
-                if (a.post) centre<VEC, TAIL, BLK>(yv, m[1] * a.inv_c, t);
+                if (a.flags & F_PRE) centre(hv, m[0] * a.inv_c, t);
+                if (a.flags & F_POST) centre(yv, m[1] * a.inv_c, t);
             }
-            float rs_y = 0.f;
             {
-                float s[4] = {0.f, 0.f, 0.f, 0.f};
-                float w[8];
-                if (a.pre) {
+                float w[E];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) w[k] = g[k] * qw[k];
-                    s[0] = dot8(hv, hv), s[1] = dot8(w, hv), s[2] = sum8(w);
+                for (int k = 0; k < E; ++k) w[k] = g[k] * qw[k];
+                s[0] = dot_e(hv, hv), s[1] = dot_e(w, hv), s[2] = dot_e(yv, yv);
+                if (FULL) s[FULL ? 3 : 0] = sum_e(w);
+            }
+            t.sum(s);
+            const float rs_y = a.flags & F_POST ? rsqrtf(s[2] * a.inv_c + a.eps) : 1.f;
+            if (a.flags & F_PRE) {
+                const float rs = rsqrtf(s[0] * a.inv_c + a.eps);
+                const float m2 = s[1] * rs * a.inv_c, m1 = FULL && (a.flags & F_LAYER) ? s[FULL ? 3 : 0] * a.inv_c : 0.f;
+                if (FULL) sums.add(S_QB, g);
+#pragma unroll
+                for (int k = 0; k < E; ++k) {
+                    const float hat = hv[k] * rs;
+                    T[k] += rs * (g[k] * qw[k] - m1 - hat * m2);
+                    g[k] *= hat;
                 }
-                if (a.post) s[3] = dot8(yv, yv);
-                t.sum(s);
-                rs_y = rsqrtf(s[3] * a.inv_c + a.eps);
-                if (a.pre) {
-                    const float rs = rsqrtf(s[0] * a.inv_c + a.eps);
-                    const float m2 = s[1] * rs * a.inv_c, m1 = a.layer ? s[2] * a.inv_c : 0.f;
+                sums.add(S_QW, g);
+            }
+            store_row(row_of<TS>(a.dx, r, a.lddx), t, T);
+            if (a.flags & F_BRANCH) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float hat = hv[k] * rs;
-                        s_qw[k] += g[k] * hat;
-                        s_qb[k] += g[k];
-                        T[k] += rs * (w[k] - m1 - hat * m2);
+                for (int k = 0; k < E; ++k) T[k] *= a.scale, yv[k] *= rs_y;
+                if (GATE == G_ROW) {
+                    float dg[E], pb[E];
+                    if (a.flags & F_POST) {
+                        load_gain(a.pb, t, pb, 0.f);
+#pragma unroll
+                        for (int k = 0; k < E; ++k) dg[k] = T[k] * (yv[k] * pw[k] + pb[k]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < E; ++k) dg[k] = T[k] * yv[k];
                     }
+#pragma unroll
+                    for (int k = 0; k < E; ++k) {
+                        const float ac = a.flags & F_SIGMOID ? sigmoid(gt[k]) : gt[k];
+                        dg[k] *= a.flags & F_SIGMOID ? ac * (1.f - ac) : 1.f;
+                        T[k] *= ac;
+                    }
+                    if (a.dgate) store_row(row_of<TB>(a.dgate, r, a.lddg), t, dg);
                 }
-            }
-            store_row<TS, VEC, TAIL, BLK>((TS*)a.dx + r * a.lddx, t, T);
-            if (!a.dy) continue;
+                if (SUM_T) sums.add(S_PB, T);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) T[k] *= a.scale;
-            if (a.post) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) yv[k] *= rs_y;
-            }
-            if (a.gate) {
-                float dg[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const float act = a.sigmoid ? sigmoid(gt[k]) : gt[k], slope = a.sigmoid ? act * (1.f - act) : 1.f;
-                    const float p = a.post ? yv[k] * pw[k] + pb[k] : yv[k];
-                    dg[k] = T[k] * p * slope;
-                    T[k] *= act;
+                for (int k = 0; k < E; ++k) {
+                    g[k] = T[k] * yv[k];
+                    if (GATE == G_SHARED) T[k] *= act[k];
                 }
-                if (shared_gate) {
+                sums.add(S_PW, g);
+                if (a.flags & F_POST) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) s_g[k] += dg[k];
-                } else if (a.dgate) {
-                    store_row<TB, VEC, TAIL, BLK>((TB*)a.dgate + r * a.lddg, t, dg);
+                    for (int k = 0; k < E; ++k) T[k] *= pw[k];       // behind the row T is what the pre norm left there, pw is 0
+                    float q[FULL ? 2 : 1] = {dot_e(T, yv)};
+                    if (FULL) q[FULL ? 1 : 0] = sum_e(T);
+                    t.sum(q);
+                    const float m2 = q[0] * a.inv_c, m1 = FULL && (a.flags & F_LAYER) ? q[FULL ? 1 : 0] * a.inv_c : 0.f;
+#pragma unroll
+                    for (int k = 0; k < E; ++k) T[k] = rs_y * (T[k] - m1 - yv[k] * m2);
                 }
-            }
-            if (a.post) {
-                float q[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    s_pw[k] += T[k] * yv[k];
-                    s_pb[k] += T[k];
-                    q[k] = T[k] * pw[k];     // beyond the row T is what the pre norm left there, pw is 0
-                }
-                float s[2] = {sum8(q), dot8(q, yv)};
-                t.sum(s);
-                const float m1 = a.layer ? s[0] * a.inv_c : 0.f, m2 = s[1] * a.inv_c;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) T[k] = rs_y * (q[k] - m1 - yv[k] * m2);
-            }
-            store_row<TB, VEC, TAIL, BLK>((TB*)a.dy + r * a.lddy, t, T);
-        }
-        if (shared_gate) {
-            if constexpr (!BLK) join_teams<VEC>(s_g, t, buf);
-            if (t.row == 0) {
-                if (a.per_group == 1)
-                    store_row<TB, VEC, TAIL, BLK>((TB*)a.dgate + group * a.lddg, t, s_g);
-                else
-                    store_row<float, VEC, TAIL, BLK>(a.gpart + (int64_t)u * a.C, t, s_g);
+                store_row(row_of<TB>(a.dy, r, a.lddy), t, T);
             }
         }
-    }
-    float* part = a.part + (int64_t)blockIdx.x * a.nslot * a.C;
-    const float(*all[4])[8] = {&s_pw, &s_pb, &s_qw, &s_qb};
+        if (GATE == G_SHARED) {
+            float v[E], w[E], pb[E];
+            sums.get(S_PW, v);
+            sums.get(S_PB, w);
+            load_gain(a.pb, t, pb, 0.f);
+            // a slot that no other sum needs takes dgate: S_PB where the bias has no gradient, else behind the rest
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (a.slot[i] < 0) continue;
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = (*all[i])[k];
-        if constexpr (!BLK) join_teams<VEC>(v, t, buf);
-        if (t.row == 0) store_row<float, VEC, TAIL, BLK>(part + (int64_t)a.slot[i] * a.C, t, v);
+            for (int k = 0; k < E; ++k) {
+                pb[k] = (a.flags & F_POST ? pw[k] * v[k] + pb[k] * w[k] : v[k]) * (a.flags & F_SIGMOID ? act[k] * (1.f - act[k]) : 1.f);
+                v[k] *= act[k], w[k] *= act[k];
+            }
+            sums.set(S_PW, v);
+            sums.set(S_PB, pb);
+            if (!BLK) __syncthreads();
+            if (a.dgate) {
+                if (a.u.per_group == 1) leave(S_PB, sums, t, lds, row_of<TB>(a.dgate, group, a.lddg), false);
+                else leave(S_PB, sums, t, lds, a.gpart + (int64_t)u * a.C, false);
+            }
+            if (FULL) {
+                if (!BLK) __syncthreads();
+                sums.set(S_PB, w);
+            }
+        }
+        if (!BLK) __syncthreads();
+        float* part = a.part + (int64_t)blockIdx.x * a.nslot * a.C;
+        const bool add = u != blockIdx.x;
+        if constexpr (BLK) {
+            if (a.slot[0] >= 0) leave(S_PW, sums, t, lds, part + (int64_t)a.slot[0] * a.C, add);
+            if (a.slot[2] >= 0) leave(S_QW, sums, t, lds, part + (int64_t)a.slot[2] * a.C, add);
+            if (FULL && a.slot[1] >= 0) leave(S_PB, sums, t, lds, part + (int64_t)a.slot[1] * a.C, add);
+            if (FULL && a.slot[3] >= 0) leave(S_QB, sums, t, lds, part + (int64_t)a.slot[3] * a.C, add);
+        } else {                     // all columns of all sums at once: few columns would leave most threads idle
+            for (int i = threadIdx.x; i < a.nslot * a.C; i += 256) {
+                const int slot = i / a.C, c = i - slot * a.C;
+                const int sum = slot == a.slot[0] ? S_PW : slot == a.slot[2] ? S_QW : slot == a.slot[1] ? S_PB : S_QB;
+                const float s = joined(sum, c, t, lds);
+                part[i] = add ? part[i] + s : s;
+            }
+            if (u + gridDim.x < a.u.units) __syncthreads();      // before the next unit's sums
+        }
     }
 }
 
@@ -403,19 +640,17 @@ __global__ void __launch_bounds__(1024) rn_join_kernel(const JoinArgs a) {
 
 // ------------------------------------------------------------------------------------------------- host
 struct Shape {
-    bool blk, tail;
+    bool blk;
+    int e, vec;                      // elements of a lane, of a vector
     int threads, tl, teams;          // threads of a workgroup, log2 of a team's lanes (rows within a wave), teams of a workgroup
 };
 
-// 16-bit tensors on both sides: a lane's 8 elements are one 16-byte vector; with fp32 on one side two vectors of 4, a team apart,
-// so that a wave's access is contiguous there too
-int vec_of(int stream_type) { return stream_type == SR_T_F32 ? 4 : 8; }
-
-Shape shape_of(int C, int vec) {
+Shape shape_of(const sr_residual_norm_desc* d, int e) {
     Shape s;
-    const int lanes = (C + 7) / 8;
-    s.blk = C > WAVE_C;
-    s.tail = C % vec != 0;
+    const int lanes = (d->channels + e - 1) / e;
+    s.e = e;
+    s.vec = d->stream_type == SR_T_F32 ? 4 : e;
+    s.blk = d->channels > WAVE_C;
     s.tl = 0;
     while (!s.blk && (1 << s.tl) < lanes) ++s.tl;
     s.threads = s.blk ? (lanes + 63) / 64 * 64 : 256;
@@ -423,29 +658,30 @@ Shape shape_of(int C, int vec) {
     return s;
 }
 
-// Work split of a backward pass: units of `chunk` rows inside one group of rows that share a gate row (without such a gate all
-// rows are one group), `blocks` workgroups over them
 struct Split {
-    unsigned span = 1, chunk = 1, per_group = 1, units = 0;
+    Units u = {1, 0, 1};
     int blocks = 0;
     bool shared_gate = false;
 };
 
-Split split_of(const sr_residual_norm_desc* d, const Shape& s, bool gate, unsigned rpg) {
+// `waves`: how many waves of the kernel a CU holds at once.  The workgroups are as many as that gives: a few more would cost a
+// second round of them, and with many more a team has too few rows to have the next one on its way (16384 x 4096 bf16 forward: 100
+// us with 16 waves a CU, 105 with 48, 112 with one row a workgroup)
+Split split_of(const sr_residual_norm_desc* d, const Shape& s, bool gate, unsigned rpg, int waves) {
     Split p;
     if (d->rows == 0) return p;
     p.shared_gate = gate && rpg > 1;
-    p.span = p.shared_gate ? rpg : (unsigned)d->rows;
-    const int64_t target = s.blk ? (s.threads > 512 ? 256 : 512) : 1024;
-    int64_t chunk = (d->rows + target - 1) / target;
-    chunk = std::min<int64_t>((chunk + s.teams - 1) / s.teams * s.teams, p.span);
-    p.chunk = (unsigned)chunk;
-    p.per_group = (unsigned)((p.span + chunk - 1) / chunk);
-    p.units = (unsigned)(d->rows / p.span * p.per_group);
-    p.blocks = (int)std::min<int64_t>(p.units, 2 * target);
+    p.u.span = p.shared_gate ? rpg : (unsigned)d->rows;
+    const int64_t groups = d->rows / p.u.span, resident = 256 * std::max(1, waves * 64 / s.threads);
+    const int64_t most = (p.u.span + s.teams - 1) / s.teams;
+    p.u.per_group = (unsigned)std::min(most, std::max<int64_t>(1, resident / groups));
+    p.u.units = (unsigned)(groups * p.u.per_group);
+    p.blocks = (int)std::min<int64_t>(p.u.units, resident);
     return p;
 }
 
+// 16-bit tensors on both sides: a lane's 8 elements are one 16-byte vector; with fp32 on one side two vectors of 4, a team apart,
+// so that a wave's access is contiguous there too
 #define RN_TYPES(LAUNCH)                                                                              \
     do {                                                                                              \
         if (d->stream_type == SR_T_BF16) LAUNCH(bf16_t, bf16_t, 8);                                   \
@@ -455,13 +691,60 @@ Split split_of(const sr_residual_norm_desc* d, const Shape& s, bool gate, unsign
         else LAUNCH(float, f16_t, 4);                                                                 \
     } while (0)
 
-#define RN_SHAPES(KERNEL, TS, TB, VEC, GRID)                                                                          \
-    do {                                                                                                              \
-        if (s.blk && s.tail) KERNEL<TS, TB, VEC, true, true><<<GRID, s.threads, 0, st>>>(a);                          \
-        else if (s.blk) KERNEL<TS, TB, VEC, false, true><<<GRID, s.threads, 0, st>>>(a);                              \
-        else if (s.tail) KERNEL<TS, TB, VEC, true, false><<<GRID, s.threads, 0, st>>>(a);                             \
-        else KERNEL<TS, TB, VEC, false, false><<<GRID, s.threads, 0, st>>>(a);                                        \
-    } while (0)
+template <typename TS, typename TB, int VEC, bool BLK, bool TAIL>
+void launch_fwd(const FwdArgs& a, int gate, int blocks, int threads, hipStream_t st) {
+    if (gate == G_NONE) rn_fwd_kernel<TS, TB, 8, VEC, BLK, TAIL, G_NONE><<<blocks, threads, 0, st>>>(a);
+    else if (gate == G_ROW) rn_fwd_kernel<TS, TB, 8, VEC, BLK, TAIL, G_ROW><<<blocks, threads, 0, st>>>(a);
+    else rn_fwd_kernel<TS, TB, 8, VEC, BLK, TAIL, G_SHARED><<<blocks, threads, 0, st>>>(a);
+}
+
+template <typename TS, typename TB, int VEC>
+void launch(const FwdArgs& a, bool blk, int gate, int blocks, int threads, hipStream_t st) {
+    if (blk && a.C % VEC) launch_fwd<TS, TB, VEC, true, true>(a, gate, blocks, threads, st);
+    else if (blk) launch_fwd<TS, TB, VEC, true, false>(a, gate, blocks, threads, st);
+    else if (a.C % VEC) launch_fwd<TS, TB, VEC, false, true>(a, gate, blocks, threads, st);
+    else launch_fwd<TS, TB, VEC, false, false>(a, gate, blocks, threads, st);
+}
+
+template <typename TS, typename TB, int E, int VEC, bool BLK, bool TAIL, int GATE, bool FULL>
+void launch_bwd(const BwdArgs& a, int blocks, int threads, hipStream_t st) {
+    const int lds = (FULL ? 16 : GATE == G_SHARED ? 12 : 8) * E * threads + (BLK ? 1024 : 0);
+    if (BLK && lds > 64 * 1024)      // a launch may have 64 KiB unless the function says more
+        (void)hipFuncSetAttribute((const void*)rn_bwd_kernel<TS, TB, E, VEC, BLK, TAIL, GATE, FULL>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    rn_bwd_kernel<TS, TB, E, VEC, BLK, TAIL, GATE, FULL><<<blocks, threads, lds, st>>>(a);
+}
+
+template <typename TS, typename TB, int E, int VEC, bool BLK, bool TAIL>
+void launch_bwd(const BwdArgs& a, int gate, bool full, int blocks, int threads, hipStream_t st) {
+    if (gate == G_NONE) full ? launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_NONE, true>(a, blocks, threads, st) : launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_NONE, false>(a, blocks, threads, st);
+    else if (gate == G_ROW) full ? launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_ROW, true>(a, blocks, threads, st) : launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_ROW, false>(a, blocks, threads, st);
+    else full ? launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_SHARED, true>(a, blocks, threads, st) : launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_SHARED, false>(a, blocks, threads, st);
+}
+
+template <typename TS, typename TB, int VEC>
+void launch(const BwdArgs& a, const Shape& s, int gate, bool full, int blocks, hipStream_t st) {
+    if (s.blk && s.e == 4) a.C % 4 ? launch_bwd<TS, TB, 4, 4, true, true>(a, gate, full, blocks, s.threads, st) : launch_bwd<TS, TB, 4, 4, true, false>(a, gate, full, blocks, s.threads, st);
+    else if (s.blk) a.C % VEC ? launch_bwd<TS, TB, 8, VEC, true, true>(a, gate, full, blocks, s.threads, st) : launch_bwd<TS, TB, 8, VEC, true, false>(a, gate, full, blocks, s.threads, st);
+    else a.C % VEC ? launch_bwd<TS, TB, 8, VEC, false, true>(a, gate, full, blocks, s.threads, st) : launch_bwd<TS, TB, 8, VEC, false, false>(a, gate, full, blocks, s.threads, st);
+}
+
+// A backward pass: the plan its workspace and its launch go by.  `full` (kernel template) is not known to the workspace query, which
+// therefore takes the larger of both.
+struct BwdPlan {
+    Shape s;
+    Split p;
+    size_t part, bytes;              // bytes of the partial sums, of everything
+};
+
+BwdPlan bwd_plan(const sr_residual_norm_desc* d, bool gate, unsigned rpg, bool full) {
+    BwdPlan q;
+    const bool simple = !full && !gate && d->channels % 8 == 0;
+    q.s = shape_of(d, d->channels <= WAVE_C || d->channels > 4096 || simple ? 8 : 4);
+    q.p = split_of(d, q.s, gate, rpg, q.s.blk || simple ? 16 : 12);
+    q.part = round_up_sz((size_t)q.p.blocks * 4 * d->channels * 4);
+    q.bytes = q.part + (q.p.shared_gate && q.p.u.per_group > 1 ? (size_t)q.p.u.units * d->channels * 4 : 0);
+    return q;
+}
 
 int check_desc(const sr_residual_norm_desc* d, const char* who) {
     if (!d) return fail(nullptr, SR_ERR_ARG, "%s: descriptor is NULL", who);
@@ -490,7 +773,7 @@ int check_gate(const sr_residual_norm_desc* d, bool gate, const char* who, unsig
 
 int region(Region* out, const void* p, int64_t rows, int64_t ld, int C, int bytes, const char* who, const char* what) {
     *out = Region{(const char*)p, p ? rows : 0, ld * bytes, (int64_t)C * bytes};
-    if (p && rows > 1 && (ld < C || ld > ((int64_t)1 << 40))) return fail(nullptr, SR_ERR_ARG, "%s: the row pitch of %s is below the channels or over 2^40", who, what);
+    if (p && rows > 1 && (ld < C || ld > INT32_MAX)) return fail(nullptr, SR_ERR_ARG, "%s: the row pitch of %s is below the channels or over 2^31 - 1", who, what);
     if (p && (uintptr_t)p % bytes) return fail(nullptr, SR_ERR_ARG, "%s: %s is not aligned to its elements", who, what);
     return SR_OK;
 }
@@ -542,13 +825,16 @@ extern "C" int sr_op_residual_norm(int device, const sr_residual_norm_desc* d, c
     OnDevice on;
     RN_TRY(on.enter(device));
     if (d->rows == 0) return SR_OK;
-    const Shape s = shape_of(C, vec_of(d->stream_type));
-    const FwdArgs a = {x, y, gate, post ? post_gain : nullptr, post ? post_bias : nullptr, pre ? pre_gain : nullptr,
-                       pre ? pre_bias : nullptr, h, n, d->ldx, d->ldy, d->ldg, d->ldh, d->ldn, (unsigned)d->rows, rpg, C, s.tl,
-                       d->kind == SR_NORM_LAYER, post, pre, d->gate_act == SR_GATE_SIGMOID, d->scale, d->eps, 1.f / (float)C};
-    const int grid = (int)std::min<int64_t>((d->rows + s.teams - 1) / s.teams, 1 << 20);
+    const Shape s = shape_of(d, 8);
+    const Split p = split_of(d, s, false, 1, 16);
+    const int flags = (y ? F_BRANCH : 0) | (post ? F_POST : 0) | (pre ? F_PRE : 0) | (d->kind == SR_NORM_LAYER ? F_LAYER : 0) |
+                      (d->gate_act == SR_GATE_SIGMOID ? F_SIGMOID : 0);
+    const FwdArgs a = {x, y, gate, post ? post_gain : nullptr, post ? post_bias : nullptr, pre ? pre_gain : nullptr, pre ? pre_bias : nullptr,
+                       h, n, (int)d->ldx, (int)d->ldy, (int)d->ldg, (int)d->ldh, (int)d->ldn, (unsigned)d->rows, rpg, C, s.tl, flags, d->scale, d->eps,
+                       1.f / (float)C};
     hipStream_t st = (hipStream_t)hip_stream;
-#define LAUNCH(TS, TB, VEC) RN_SHAPES(rn_fwd_kernel, TS, TB, VEC, grid)
+    const int gt = !gate ? G_NONE : rpg > 1 ? G_SHARED : G_ROW;
+#define LAUNCH(TS, TB, VEC) launch<TS, TB, VEC>(a, s.blk, gt, p.blocks, s.threads, st)
     RN_TYPES(LAUNCH);
 #undef LAUNCH
     const hipError_t e = hipGetLastError();
@@ -562,9 +848,7 @@ extern "C" int sr_op_residual_norm_bwd_workspace(const sr_residual_norm_desc* d,
     if (!bytes) return fail(nullptr, SR_ERR_ARG, "%s: bytes is NULL", who);
     unsigned rpg;
     RN_TRY(check_gate(d, gate != 0, who, &rpg));
-    const Split p = split_of(d, shape_of(d->channels, vec_of(d->stream_type)), gate != 0, rpg);
-    const size_t row = (size_t)d->channels * 4;
-    *bytes = round_up_sz((size_t)p.blocks * 4 * row) + (p.shared_gate && p.per_group > 1 ? (size_t)p.units * row : 0);
+    *bytes = std::max(bwd_plan(d, gate != 0, rpg, false).bytes, bwd_plan(d, gate != 0, rpg, true).bytes);
     return SR_OK;
 }
 
@@ -622,26 +906,30 @@ extern "C" int sr_op_residual_norm_bwd(int device, const sr_residual_norm_desc* 
     OnDevice on;
     RN_TRY(on.enter(device));
     hipStream_t st = (hipStream_t)hip_stream;
-    const Shape s = shape_of(C, vec_of(d->stream_type));
-    const Split p = split_of(d, s, gate != nullptr, rpg);
+    const bool full = d->kind == SR_NORM_LAYER || dpost_bias || dpre_bias;
+    const BwdPlan q = bwd_plan(d, gate != nullptr, rpg, full);
+    const Split& p = q.p;
     float* part = (float*)workspace;
-    float* gpart = (float*)((char*)workspace + round_up_sz((size_t)p.blocks * 4 * C * 4));
-    JoinArgs j = {part, {}, p.blocks, 0, {-1, -1, -1, -1}, C, gpart, dgate, d->lddg, (int)p.per_group, d->branch_type};
+    float* gpart = (float*)((char*)workspace + q.part);
+    JoinArgs j = {part, {}, p.blocks, 0, {-1, -1, -1, -1}, C, gpart, dgate, d->lddg, (int)p.u.per_group, d->branch_type};
     for (int i = 0; i < 4; ++i) {
         j.out[i] = vec[i];
         if (vec[i]) j.slot[i] = j.nslot++;
     }
     if (d->rows) {
+        const int flags = (dy ? F_BRANCH : 0) | (post ? F_POST : 0) | (pre ? F_PRE : 0) | (d->kind == SR_NORM_LAYER ? F_LAYER : 0) |
+                          (d->gate_act == SR_GATE_SIGMOID ? F_SIGMOID : 0) | (dh ? F_STREAM_GRAD : 0) | (y ? F_READ_Y : 0);
         const BwdArgs a = {h, y, gate, dh, dn, post ? post_gain : nullptr, post ? post_bias : nullptr, pre ? pre_gain : nullptr, dx, dy, dgate,
-                           part, gpart, d->ldh, d->ldy, d->ldg, d->lddh, d->lddn, d->lddx, d->lddy, d->lddg, p.span,
-                           p.units, p.chunk, p.per_group, gate && rpg == 1, C, s.tl, d->kind == SR_NORM_LAYER, post, pre, d->gate_act == SR_GATE_SIGMOID,
-                           j.nslot, {j.slot[0], j.slot[1], j.slot[2], j.slot[3]}, d->scale, d->eps, 1.f / (float)C};
-#define LAUNCH(TS, TB, VEC) RN_SHAPES(rn_bwd_kernel, TS, TB, VEC, p.blocks)
+                           part, gpart, (int)d->ldh, (int)d->ldy, (int)d->ldg, (int)d->lddh, (int)d->lddn, (int)d->lddx, (int)d->lddy,
+                           (int)d->lddg, p.u, C, q.s.tl, flags, j.nslot, {j.slot[0], j.slot[1], j.slot[2], j.slot[3]}, d->scale, d->eps,
+                           1.f / (float)C};
+        const int gt = !gate ? G_NONE : p.shared_gate ? G_SHARED : G_ROW;
+#define LAUNCH(TS, TB, VEC) launch<TS, TB, VEC>(a, q.s, gt, full, p.blocks, st)
         RN_TYPES(LAUNCH);
 #undef LAUNCH
     }
     hipError_t e = hipGetLastError();
-    const unsigned gates = dgate && p.shared_gate && p.per_group > 1 ? (unsigned)(d->rows / rpg) : 0;
+    const unsigned gates = dgate && p.shared_gate && p.u.per_group > 1 ? (unsigned)(d->rows / rpg) : 0;
     if (e == hipSuccess && (j.nslot || gates)) {
         rn_join_kernel<<<dim3((C + 15) / 16, 4 + gates), 1024, 0, st>>>(j);
         e = hipGetLastError();
