@@ -439,7 +439,7 @@ int sr_op_residual_norm_bwd(int device, const sr_residual_norm_desc* desc, const
 
 /* A list of dense tensors on one device (a model's gradients): `count` elements of enum sr_type `type` from `data` on, aligned to
  * their elements; count may be 0.  The list holds addresses, not memory: it is valid as long as the tensors stay where they are, and
- * may be used by several threads.  sr_tensors_workspace: bytes of workspace (8-byte aligned) the calls below need. */
+ * may be used by several threads (not while sr_tensors_upload runs).  sr_tensors_workspace: bytes of workspace (8-byte aligned) the calls below need. */
 typedef struct sr_tensors sr_tensors;
 typedef struct sr_tensor_desc {
     void* data;
@@ -447,6 +447,9 @@ typedef struct sr_tensor_desc {
     int32_t type;
 } sr_tensor_desc;
 int sr_tensors_create(sr_tensors** out, int device, int n, const sr_tensor_desc* tensors);
+/* Leaves a record of every part of the list in device memory that the list owns; later calls with lists of more than 160 tensors then need no launches to write them, and others start a little
+ * sooner.  Synchronous, not during a capture; calls that are captured do not use the records, so a graph may outlive the list. */
+int sr_tensors_upload(sr_tensors* t);
 int sr_tensors_destroy(sr_tensors* t);
 int sr_tensors_workspace(const sr_tensors* t, size_t* bytes);
 /* d_norm (one float) = scale * sqrt(sum of the squares of all elements), d_norms (nullable, one float a tensor) = the same of each

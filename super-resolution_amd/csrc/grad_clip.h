@@ -6,8 +6,8 @@
 
 namespace sr {
 
-constexpr int GRAD_PARTS = 2048;    // partial sums of a list of n pieces: at most GRAD_PARTS + n
-constexpr uint32_t GRAD_PIECE = 1u << 30;   // elements of a piece: longer tensors are several pieces
+constexpr int GRAD_PARTS = 4096;    // partial sums of a list of n pieces: at most GRAD_PARTS + n
+constexpr uint32_t GRAD_PIECE = 1u << 29;   // elements of a piece: longer tensors are several pieces
 
 // a run of `n` <= GRAD_PIECE dense elements of enum sr_type `type`
 struct GradPiece {
@@ -18,7 +18,7 @@ struct GradPiece {
 // elements of one partial sum, so that `total` elements make at most GRAD_PARTS full ones
 uint32_t grad_chunk(int64_t total);
 inline int64_t grad_chunks(uint32_t n, uint32_t chunk) { return ((int64_t)n + chunk - 1) / chunk; }
-// parts[i] = sum of squares of chunk i; piece after piece, the chunks of a piece in order.  Writes every part it counts.
+// parts[i] = sum of squares of chunk i; piece after piece, the chunks of a piece in order.  At most 160 pieces.
 hipError_t launch_grad_partials(const GradPiece* pieces, int n, uint32_t chunk, double* parts, hipStream_t s);
 
 // What a kernel needs to know the norm of scaled gradients: two runs of partial sums (the second may be empty) and their scales
@@ -34,6 +34,7 @@ struct ClipArgs {
 __device__ __forceinline__ float clip_factor(const ClipArgs& c, double* lds4) {
     double s = 0.0;
     const double q0 = (double)c.s0 * c.s0, q1 = (double)c.s1 * c.s1;
+#pragma unroll 8
     for (int i = threadIdx.x; i < c.n0 + c.n1; i += 256) s += c.parts[i] * (i < c.n0 ? q0 : q1);
     for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
     if ((threadIdx.x & 63) == 0) lds4[threadIdx.x >> 6] = s;

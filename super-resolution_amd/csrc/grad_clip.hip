@@ -4,16 +4,16 @@
 //
 // Bound by HBM: the norm reads every gradient once, clipping reads it again (from the 256 MB last-level cache where it is still
 // there) and writes it once.  The squares are added in 64 bits: an fp32 square overflows above 1.8e19 and vanishes below 1e-23, a
-// 64-bit one does neither, and beside the loads the conversions and products cost nothing.  A tensor is cut into chunks, a workgroup
-// takes one chunk and leaves one partial sum; chunks grow with the whole list so that there are about 2048 of them at most, which
-// every workgroup of the clipping launch adds up by itself in one fixed order (2048 doubles from L2) -- no atomics, no third
-// launch, the same bits on every run.  The chunk table travels in the kernel arguments: nothing is uploaded, and a captured
-// graph holds its own copy.
+// 64-bit one does neither, and beside the loads the conversions and products cost nothing (250 M bf16 elements: 84 us, 5.9 TB/s).
+// A tensor is cut into chunks, a workgroup takes one chunk and leaves one partial sum; chunks grow with the whole list so that there
+// are about 4096 of them at most, which every workgroup of the clipping launch adds up by itself in one fixed order (32 KB from L2)
+// -- no atomics, no third launch, the same bits on every run.
 #include "grad_clip.h"
 #include "op_host.h"
 #include "row_math.h"
 
 #include <algorithm>
+#include <mutex>
 #include <new>
 
 using namespace sr;
@@ -21,37 +21,66 @@ using namespace srh;
 
 namespace {
 
-// 224 x (8 + 4 + 4 + 1) and 152 x (16 + 4 + 4 + 1) bytes of the 4 KiB of kernel arguments
-constexpr int NORM_MAX = 224, SCALE_MAX = 152;
-
-template <int MAX>
-struct Pieces {
-    uint32_t n[MAX], first[MAX];    // elements of a piece, its first chunk in this launch
-    uint8_t type[MAX];
+// Where a workgroup finds its chunk.  A list of up to TABLE pieces travels in the kernel arguments (24 bytes a piece of their
+// 4 KiB): nothing is uploaded, and a captured graph holds its own copy.  Longer ones have a record for every chunk in device memory,
+// so that a pass is one launch whatever the number of tensors: in memory of the list where sr_tensors_upload has left them, or in
+// the workspace, where a launch for every TABLE pieces (4.7 us each, mostly the way of the arguments) writes them first.  Clipping
+// 60 M elements in 700 tensors took 188 us with a launch for every 224 or 152 pieces.
+constexpr int TABLE = 160;
+struct Piece {
+    const void* src;
+    void* dst;
+    uint32_t n, first;              // elements, with the type in the two highest bits; the piece's first chunk
+};
+struct Table {
+    Piece e[TABLE];
     int count;
     uint32_t chunk;
+};
+static_assert(sizeof(Table) + sizeof(ClipArgs) + 64 <= 4096, "kernel arguments");
 
-    // the piece that owns chunk b of this launch
-    __device__ __forceinline__ int find(uint32_t b) const {
-        int lo = 0, hi = count - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (first[mid] <= b) lo = mid;
-            else hi = mid - 1;
-        }
-        return lo;
+struct Record {
+    const char* p;
+    uint32_t n, type;
+};
+struct Records {
+    const Record *src, *dst;
+};
+
+struct Chunk {
+    const char* src;
+    char* dst;
+    uint32_t n, type;
+};
+__device__ __forceinline__ Chunk chunk_of(const Piece& e, uint32_t b, uint32_t chunk) {
+    const uint32_t at = (b - e.first) * chunk, n = e.n & 0x3fffffffu, type = e.n >> 30;
+    const size_t bytes = (size_t)at * (type == SR_T_F32 ? 4 : 2);
+    return {(const char*)e.src + bytes, (char*)e.dst + bytes, min(chunk, n - at), type};
+}
+__device__ __forceinline__ Chunk chunk_of(const Table& t, uint32_t b) {
+    // the last piece that does not start behind chunk b: every lane of the wave compares a few
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < (TABLE + 63) / 64; ++i) {
+        const int k = i * 64 + (threadIdx.x & 63);
+        before += __popcll(__ballot(k < t.count && t.e[k < TABLE ? k : 0].first <= b));
     }
-};
+    return chunk_of(t.e[__builtin_amdgcn_readfirstlane(before) - 1], b, t.chunk);
+}
+__device__ __forceinline__ Chunk chunk_of(const Records& t, uint32_t b) {
+    const Record s = t.src[b];
+    return {s.p, (char*)t.dst[b].p, s.n, s.type};
+}
 
-struct NormTable {
-    const void* src[NORM_MAX];
-    Pieces<NORM_MAX> p;
-};
-struct ScaleTable {
-    const void* src[SCALE_MAX];
-    void* dst[SCALE_MAX];
-    Pieces<SCALE_MAX> p;
-};
+__global__ void __launch_bounds__(64) grad_records_kernel(const Table t, Record* __restrict__ src, Record* __restrict__ dst) {
+    const Piece e = t.e[blockIdx.x];
+    const uint32_t chunks = ((e.n & 0x3fffffffu) + t.chunk - 1) / t.chunk;
+    for (uint32_t i = threadIdx.x; i < chunks; i += 64) {
+        const Chunk c = chunk_of(e, e.first + i, t.chunk);
+        src[e.first + i] = {c.src, c.n, c.type};
+        dst[e.first + i] = {c.dst, c.n, c.type};
+    }
+}
 
 __device__ __forceinline__ double block_sum(double s, double* lds4) {
     for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
@@ -78,41 +107,35 @@ __device__ __forceinline__ double sum_squares(const T* p, uint32_t n) {
     return s[0] + s[1];
 }
 
-__global__ void __launch_bounds__(256) grad_partials_kernel(const NormTable t, double* __restrict__ parts) {
+template <typename TABLE_T>
+__global__ void __launch_bounds__(256) grad_partials_kernel(const TABLE_T t, double* __restrict__ parts) {
     __shared__ double lds4[4];
-    const int e = t.p.find(blockIdx.x);
-    const uint32_t at = (blockIdx.x - t.p.first[e]) * t.p.chunk, n = min(t.p.chunk, t.p.n[e] - at);
+    const Chunk c = chunk_of(t, blockIdx.x);
     double s;
-    if (t.p.type[e] == SR_T_F32) s = sum_squares((const float*)t.src[e] + at, n);
-    else if (t.p.type[e] == SR_T_BF16) s = sum_squares((const bf16_t*)t.src[e] + at, n);
-    else s = sum_squares((const f16_t*)t.src[e] + at, n);
+    if (c.type == SR_T_F32) s = sum_squares((const float*)c.src, c.n);
+    else if (c.type == SR_T_BF16) s = sum_squares((const bf16_t*)c.src, c.n);
+    else s = sum_squares((const f16_t*)c.src, c.n);
     s = block_sum(s, lds4);
     if (threadIdx.x == 0) parts[blockIdx.x] = s;
 }
 
-// workgroup 0: the norm of everything; the others: one tensor a wave
+// workgroup 0: the norm of everything; the others: a tensor each
 constexpr int EACH_MAX = 900;
 struct EachTable {
     uint32_t first[EACH_MAX + 1];   // partial sums of the tensors of this launch
     int count;
 };
-__global__ void __launch_bounds__(256) grad_norm_kernel(const EachTable t, const double* __restrict__ parts, int nparts, float scale,
+__global__ void __launch_bounds__(256) grad_norm_kernel(const EachTable t, const double* __restrict__ parts, uint32_t nparts, float scale,
                                                         float* __restrict__ norm, float* __restrict__ each) {
     __shared__ double lds4[4];
-    if (blockIdx.x == 0) {
-        if (!norm) return;
-        double s = 0.0;
-        for (int i = threadIdx.x; i < nparts; i += 256) s += parts[i];
-        s = block_sum(s, lds4);
-        if (threadIdx.x == 0) *norm = (float)(sqrt(s) * (double)scale);
-        return;
-    }
-    const int i = ((int)blockIdx.x - 1) * 4 + (threadIdx.x >> 6);
-    if (i >= t.count) return;
+    const int i = (int)blockIdx.x - 1;
+    if (i < 0 && !norm) return;
+    const uint32_t k0 = i < 0 ? 0 : t.first[i], k1 = i < 0 ? nparts : t.first[i + 1];
     double s = 0.0;
-    for (uint32_t k = t.first[i] + (threadIdx.x & 63); k < t.first[i + 1]; k += 64) s += parts[k];
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-    if ((threadIdx.x & 63) == 0) each[i] = (float)(sqrt(s) * (double)scale);
+#pragma unroll 16
+    for (uint32_t k = k0 + threadIdx.x; k < k1; k += 256) s += parts[k];
+    s = block_sum(s, lds4);
+    if (threadIdx.x == 0) *(i < 0 ? norm : each + i) = (float)(sqrt(s) * (double)scale);
 }
 
 template <typename T>
@@ -131,15 +154,15 @@ __device__ __forceinline__ void scale_run(const T* src, T* dst, uint32_t n, floa
     if (t < n) dst[t] = (T)((float)src[t] * f);
 }
 
-__global__ void __launch_bounds__(256) grad_scale_kernel(const ScaleTable t, const ClipArgs c) {
+template <typename TABLE_T>
+__global__ void __launch_bounds__(256) grad_scale_kernel(const TABLE_T t, const ClipArgs a) {
     __shared__ double lds4[4];
-    const float f = clip_factor(c, lds4) * c.s0;
-    const int e = t.p.find(blockIdx.x);
-    if (f == 1.f && t.src[e] == t.dst[e]) return;   // in place and nothing to do
-    const uint32_t at = (blockIdx.x - t.p.first[e]) * t.p.chunk, n = min(t.p.chunk, t.p.n[e] - at);
-    if (t.p.type[e] == SR_T_F32) scale_run((const float*)t.src[e] + at, (float*)t.dst[e] + at, n, f);
-    else if (t.p.type[e] == SR_T_BF16) scale_run((const bf16_t*)t.src[e] + at, (bf16_t*)t.dst[e] + at, n, f);
-    else scale_run((const f16_t*)t.src[e] + at, (f16_t*)t.dst[e] + at, n, f);
+    const Chunk c = chunk_of(t, blockIdx.x);
+    const float f = clip_factor(a, lds4) * a.s0;
+    if (f == 1.f && c.src == c.dst) return;   // in place and nothing to do
+    if (c.type == SR_T_F32) scale_run((const float*)c.src, (float*)c.dst, c.n, f);
+    else if (c.type == SR_T_BF16) scale_run((const bf16_t*)c.src, (bf16_t*)c.dst, c.n, f);
+    else scale_run((const f16_t*)c.src, (f16_t*)c.dst, c.n, f);
 }
 
 // an empty list has no chunks, but still a norm
@@ -155,24 +178,19 @@ uint32_t grad_chunk(int64_t total) {
 }
 
 hipError_t launch_grad_partials(const GradPiece* pieces, int n, uint32_t chunk, double* parts, hipStream_t s) {
-    NormTable t;
-    for (int i = 0; i < n;) {
-        uint32_t blocks = 0;
-        int k = 0;
-        for (; i < n && k < NORM_MAX; ++i) {
-            if (!pieces[i].n) continue;
-            t.src[k] = pieces[i].src, t.p.n[k] = pieces[i].n, t.p.first[k] = blocks, t.p.type[k] = (uint8_t)pieces[i].type;
-            blocks += (uint32_t)grad_chunks(pieces[i].n, chunk);
-            ++k;
-        }
-        if (!k) break;
-        t.p.count = k, t.p.chunk = chunk;
-        grad_partials_kernel<<<blocks, 256, 0, s>>>(t, parts);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-        parts += blocks;
+    Table t;
+    uint32_t blocks = 0;
+    int k = 0;
+    for (int i = 0; i < n; ++i) {
+        if (!pieces[i].n) continue;
+        if (k == TABLE) return hipErrorInvalidValue;
+        t.e[k++] = {pieces[i].src, nullptr, pieces[i].n | pieces[i].type << 30, blocks};
+        blocks += (uint32_t)grad_chunks(pieces[i].n, chunk);
     }
-    return hipSuccess;
+    if (!k) return hipSuccess;
+    t.count = k, t.chunk = chunk;
+    grad_partials_kernel<<<blocks, 256, 0, s>>>(t, parts);
+    return hipGetLastError();
 }
 
 }  // namespace sr
@@ -181,11 +199,12 @@ hipError_t launch_grad_partials(const GradPiece* pieces, int n, uint32_t chunk, 
 struct sr_tensors {
     int device = 0;
     std::vector<sr_tensor_desc> list;
-    std::vector<GradPiece> pieces;
+    std::vector<Piece> pieces;               // dst: the tensor itself
     std::vector<uint32_t> first;             // first partial sum of every tensor, and their number
     std::vector<std::pair<const char*, const char*>> sorted;   // byte ranges by address
     uint32_t chunk = 0;
     bool overlap = false;                    // two tensors share memory
+    Record* d_records = nullptr;             // of every chunk (sr_tensors_upload)
 };
 
 #define GC_TRY(call)          \
@@ -196,7 +215,57 @@ struct sr_tensors {
 
 namespace {
 
-size_t workspace_of(const sr_tensors* t) { return std::max<size_t>(t->first.back(), 1) * sizeof(double); }
+// Records of lists that are gone.  They are freed by the next upload on their device: hipFree waits for the calls that may still read
+// them, and would end a capture that happens to be under way where a list goes out of scope.
+std::mutex g_retired_mu;
+std::vector<std::pair<int, Record*>> g_retired;
+
+// workspace: the partial sums; for a list that does not fit the kernel arguments, the records of both sides
+size_t parts_bytes(const sr_tensors* t) { return std::max<size_t>(t->first.back(), 1) * sizeof(double); }
+size_t workspace_of(const sr_tensors* t) {
+    return parts_bytes(t) + (t->pieces.size() > TABLE ? 2 * t->first.back() * sizeof(Record) : 0);
+}
+
+// The kernel arguments for pieces [at, at + count) of t, written to out's tensors
+void fill(Table& a, const sr_tensors* t, const sr_tensors* out, size_t at) {
+    a.count = (int)std::min<size_t>(t->pieces.size() - at, TABLE);
+    a.chunk = t->chunk;
+    for (int i = 0; i < a.count; ++i) {
+        a.e[i] = t->pieces[at + i];
+        a.e[i].dst = out->pieces[at + i].dst;
+    }
+}
+
+// Partial sums of the whole list, and with `c` the scaled gradients.  A captured call does not go by the list's own records: a graph
+// may outlive the list.
+hipError_t launch_list(const sr_tensors* t, const sr_tensors* out, void* ws, const ClipArgs* c, hipStream_t st) {
+    const uint32_t blocks = t->first.back();
+    if (!blocks) return hipSuccess;
+    auto run = [&](const auto& table) {
+        grad_partials_kernel<<<blocks, 256, 0, st>>>(table, (double*)ws);
+        if (c) grad_scale_kernel<<<blocks, 256, 0, st>>>(table, *c);
+        return hipGetLastError();
+    };
+    Records r = {t->d_records, out->d_records};
+    if (r.src && r.dst) {
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        const hipError_t e = hipStreamIsCapturing(st, &capture);
+        if (e != hipSuccess) return e;
+        if (capture == hipStreamCaptureStatusNone) return run(r);
+    }
+    Table a;
+    if (t->pieces.size() <= TABLE) {
+        fill(a, t, out, 0);
+        return run(a);
+    }
+    Record *src = (Record*)((char*)ws + parts_bytes(t)), *dst = src + blocks;
+    for (size_t at = 0; at < t->pieces.size(); at += TABLE) {
+        fill(a, t, out, at);
+        grad_records_kernel<<<a.count, 64, 0, st>>>(a, src, dst);
+    }
+    r = {src, dst};
+    return run(r);
+}
 
 int check_call(const sr_tensors* t, float scale, const float* d_norm, const float* d_norms, const void* ws, size_t ws_bytes, const char* who) {
     if (!t) return fail(nullptr, SR_ERR_ARG, "%s: the tensor list is NULL", who);
@@ -255,7 +324,7 @@ int sr_tensors_create(sr_tensors** out, int device, int n, const sr_tensor_desc*
             const int b = type_bytes(d.type);
             for (int64_t at = 0; at < d.count; at += GRAD_PIECE) {
                 const uint32_t m = (uint32_t)std::min<int64_t>(d.count - at, GRAD_PIECE);
-                t->pieces.push_back({(const char*)d.data + at * b, m, (uint32_t)d.type});
+                t->pieces.push_back({(const char*)d.data + at * b, (char*)d.data + at * b, m | (uint32_t)d.type << 30, parts});
                 parts += (uint32_t)grad_chunks(m, t->chunk);
             }
             t->first.push_back(parts);
@@ -271,7 +340,51 @@ int sr_tensors_create(sr_tensors** out, int device, int n, const sr_tensor_desc*
     return SR_OK;
 }
 
+int sr_tensors_upload(sr_tensors* t) {
+    const char* who = "sr_tensors_upload";
+    if (!t) return fail(nullptr, SR_ERR_ARG, "%s: the tensor list is NULL", who);
+    OnDevice on;
+    GC_TRY(on.enter(t->device));
+    {
+        std::lock_guard<std::mutex> lock(g_retired_mu);
+        auto gone = std::remove_if(g_retired.begin(), g_retired.end(), [&](const std::pair<int, Record*>& r) {
+            return r.first == t->device && hipFree(r.second) == hipSuccess;
+        });
+        g_retired.erase(gone, g_retired.end());
+    }
+    const size_t n = t->first.back();
+    if (t->d_records || !n) return SR_OK;
+    try {
+        std::vector<Record> r;
+        r.reserve(n);
+        for (const Piece& p : t->pieces) {
+            const uint32_t all = p.n & 0x3fffffffu, type = p.n >> 30;
+            for (uint32_t at = 0; at < all; at += t->chunk)
+                r.push_back({(const char*)p.src + (size_t)at * type_bytes((int)type), std::min(t->chunk, all - at), type});
+        }
+        Record* d = nullptr;
+        HIPCHK(nullptr, hipMalloc((void**)&d, n * sizeof(Record)));
+        const hipError_t e = hipMemcpy(d, r.data(), n * sizeof(Record), hipMemcpyHostToDevice);
+        if (e != hipSuccess) {
+            (void)hipFree(d);
+            return fail(nullptr, SR_ERR_HIP, "%s: hipMemcpy failed: %s", who, hipGetErrorString(e));
+        }
+        t->d_records = d;
+    } catch (const std::bad_alloc&) {
+        return fail(nullptr, SR_ERR_ARG, "%s: out of host memory", who);
+    }
+    return SR_OK;
+}
+
 int sr_tensors_destroy(sr_tensors* t) {
+    if (!t) return SR_OK;
+    if (t->d_records) {
+        std::lock_guard<std::mutex> lock(g_retired_mu);
+        try {
+            g_retired.emplace_back(t->device, t->d_records);
+        } catch (const std::bad_alloc&) {    // they stay until the process ends
+        }
+    }
     delete t;
     return SR_OK;
 }
@@ -293,13 +406,13 @@ int sr_op_grad_norm(const sr_tensors* t, float scale, float* d_norm, float* d_no
     GC_TRY(on.enter(t->device));
     hipStream_t st = (hipStream_t)hip_stream;
     double* parts = (double*)workspace;
-    GC_TRY(launched(launch_grad_partials(t->pieces.data(), (int)t->pieces.size(), t->chunk, parts, st), who));
+    GC_TRY(launched(launch_list(t, t, workspace, nullptr, st), who));
     EachTable e;
     size_t at = 0;
     do {
         e.count = d_norms ? (int)std::min<size_t>(n - at, EACH_MAX) : 0;
         for (int i = 0; i <= e.count; ++i) e.first[i] = t->first[at + i];
-        grad_norm_kernel<<<1 + (e.count + 3) / 4, 256, 0, st>>>(e, parts, (int)t->first.back(), scale, at ? nullptr : d_norm, d_norms + at);
+        grad_norm_kernel<<<1 + e.count, 256, 0, st>>>(e, parts, t->first.back(), scale, at ? nullptr : d_norm, d_norms + at);
         GC_TRY(launched(hipGetLastError(), who));
         at += e.count;
     } while (d_norms && at < n);
@@ -344,29 +457,12 @@ int sr_op_clip_grads(const sr_tensors* t, const sr_tensors* out, float max_norm,
     OnDevice on;
     GC_TRY(on.enter(t->device));
     hipStream_t st = (hipStream_t)hip_stream;
-    double* parts = (double*)workspace;
-    const int n = (int)t->pieces.size();
-    if (!n) {
+    if (t->pieces.empty()) {
         grad_zero_norm_kernel<<<1, 1, 0, st>>>(d_norm);
         return launched(hipGetLastError(), who);
     }
-    GC_TRY(launched(launch_grad_partials(t->pieces.data(), n, t->chunk, parts, st), who));
-    ClipArgs c = {parts, (int)t->first.back(), 0, scale, 0.f, max_norm, d_norm};
-    ScaleTable s;
-    for (int i = 0; i < n;) {
-        uint32_t blocks = 0;
-        int k = 0;
-        for (; i < n && k < SCALE_MAX; ++i, ++k) {
-            const GradPiece& p = t->pieces[i];
-            s.src[k] = p.src, s.dst[k] = const_cast<void*>(out->pieces[i].src), s.p.n[k] = p.n, s.p.first[k] = blocks, s.p.type[k] = (uint8_t)p.type;
-            blocks += (uint32_t)grad_chunks(p.n, t->chunk);
-        }
-        s.p.count = k, s.p.chunk = t->chunk;
-        grad_scale_kernel<<<blocks, 256, 0, st>>>(s, c);
-        GC_TRY(launched(hipGetLastError(), who));
-        c.norm = nullptr;
-    }
-    return SR_OK;
+    const ClipArgs c = {(const double*)workspace, (int)t->first.back(), 0, scale, 0.f, max_norm, d_norm};
+    return launched(launch_list(t, out, workspace, &c, st), who);
 }
 
 }  // extern "C"

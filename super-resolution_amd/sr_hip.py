@@ -8,6 +8,7 @@ from __future__ import annotations
 import collections
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -115,6 +116,7 @@ SIGNATURES = {
     "sr_op_residual_norm_bwd_workspace": (C.c_int, [_vp, C.c_int, C.POINTER(C.c_size_t)]),
     "sr_op_residual_norm_bwd": (C.c_int, [C.c_int] + [_vp] * 17 + [C.c_size_t, _vp]),
     "sr_tensors_create": (C.c_int, [C.POINTER(_vp), C.c_int, C.c_int, _vp]),
+    "sr_tensors_upload": (C.c_int, [_vp]),
     "sr_tensors_destroy": (C.c_int, [_vp]),
     "sr_tensors_workspace": (C.c_int, [_vp, C.POINTER(C.c_size_t)]),
     "sr_op_grad_norm": (C.c_int, [_vp, C.c_float, _vp, _vp, _vp, C.c_size_t, _vp]),
@@ -880,13 +882,9 @@ _KINDS = {"rms": 0, "layer": 1}
 _GATES = {"linear": 0, "sigmoid": 1}
 _torch = None
 _torch_types = None
-
-
-class _ResidualNormDesc(C.Structure):
-    _fields_ = ([("rows", C.c_int64), ("rows_per_gate", C.c_int64)]
-                + [(n, C.c_int64) for n in ("ldx", "ldy", "ldg", "ldh", "ldn", "lddh", "lddn", "lddx", "lddy", "lddg")]
-                + [(n, C.c_int32) for n in ("channels", "stream_type", "branch_type", "kind", "norms", "gate_act")]
-                + [("scale", C.c_float), ("eps", C.c_float)])
+_current_stream = None
+# sr_residual_norm_desc: rows, rows_per_gate, ten pitches; channels, stream_type, branch_type, kind, norms, gate_act; scale, eps
+_pack_block = struct.Struct("=12q6i2f").pack
 
 
 class _TensorDesc(C.Structure):
@@ -894,35 +892,41 @@ class _TensorDesc(C.Structure):
 
 
 def _types():
-    global _torch, _torch_types
+    global _torch, _torch_types, _current_stream
     if _torch_types is None:
         import torch
-        _torch, _torch_types = torch, {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+        _torch = torch
+        # the handle itself where torch gives it: current_stream builds an object for it, a microsecond of a small call
+        _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda i: torch.cuda.current_stream(i).cuda_stream)
+        _torch_types = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
     return _torch_types
 
 
-def _type_of(t, what):
-    code = _types().get(t.dtype)
+def _type_of(dtype, what):
+    code = _types().get(dtype)
     if code is None:
-        raise ValueError(f"{what}: float32, bfloat16 or float16, got {t.dtype}")
+        raise ValueError(f"{what}: float32, bfloat16 or float16, got {dtype}")
     return code
 
 
-def _stream_of(stream, device):
-    """The hipStream_t of a call: the caller's (an int), or torch's current stream of that device."""
-    return _torch.cuda.current_stream(device).cuda_stream if stream is None else int(stream)
+def _on(stream, device):
+    """torch's current stream made `stream` (a hipStream_t): what the call allocates then belongs to the stream it runs on."""
+    _types()
+    return _torch.cuda.stream(_torch.cuda.ExternalStream(int(stream), device=device))
 
 
-def _rows_of(t, what, C_, device, dtype=None, rows=None):
-    """Elements between the rows of t (..., C) seen as a matrix; the checks every tensor of a call goes through."""
-    if t.device != device:
-        raise ValueError(f"{what} is on {t.device}, the call on {device}")
-    if t.dim() == 0 or t.shape[-1] != C_:
-        raise ValueError(f"{what}: expected {C_} channels in the last dimension, got shape {tuple(t.shape)}")
-    if dtype is not None and t.dtype != dtype:
+def _pitch(t, what, shape, dtype, dev):
+    """Elements between the rows of t (..., C), as many as `shape` has, seen as a matrix; the checks every tensor of a call goes
+    through.  dev: the device's number."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous():
+        return shape[-1]
+    C_ = shape[-1]
+    if t.get_device() != dev:
+        raise ValueError(f"{what} is on {t.device}, the call on cuda:{dev}")
+    if t.dtype != dtype:
         raise ValueError(f"{what}: expected {dtype}, got {t.dtype}")
-    if rows is not None and t.numel() != rows * C_:
-        raise ValueError(f"{what}: expected {rows} rows of {C_}, got shape {tuple(t.shape)}")
+    if t.dim() == 0 or t.shape[-1] != C_ or t.numel() != shape.numel():
+        raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.is_contiguous():
         return C_
     if C_ > 1 and t.stride(-1) != 1:
@@ -933,38 +937,42 @@ def _rows_of(t, what, C_, device, dtype=None, rows=None):
         raise ValueError(f"{what}: the rows of shape {tuple(t.shape)} and strides {tuple(t.stride())} are not evenly spaced") from None
 
 
-def _vector(t, what, C_, device):
+def _vector(t, what, C_, dev):
     if t is None:
         return None
-    if t.device != device or t.dtype != _torch.float32 or t.shape != (C_,) or not t.is_contiguous():
-        raise ValueError(f"{what}: expected a contiguous float32 vector of {C_} on {device}")
+    if t.dtype is not _torch.float32 or t.get_device() != dev or t.dim() != 1 or t.numel() != C_ or not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous float32 vector of {C_} on cuda:{dev}")
     return t.data_ptr()
 
 
-def _at(t):
-    return None if t is None else t.data_ptr()
-
-
-def _block(x, branch_dtype, gate, norms, kind, gate_act, scale, eps):
-    """(descriptor, rows, channels, device, pitch of the gate) of a residual-block call on x, the stream."""
-    if x.device.type != "cuda":
+def _block(x, norms, kind, gate_act):
+    """(shape, rows, device number, type, mask of norms) of a residual-block call on x, the stream."""
+    code = _type_of(x.dtype, "the stream")
+    dev = x.get_device()
+    if dev < 0:
         raise ValueError(f"the stream is on {x.device}: these operators have no CPU fallback")
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"expected (..., channels), got shape {tuple(x.shape)}")
+    shape = x.shape
+    if not shape or not shape[-1]:
+        raise ValueError(f"expected (..., channels), got shape {tuple(shape)}")
     if norms not in _NORMS or kind not in _KINDS or gate_act not in _GATES:
         raise ValueError(f"norms one of {sorted(_NORMS)}, kind one of {sorted(_KINDS)}, gate_act one of {sorted(_GATES)}")
-    C_ = x.shape[-1]
-    rows, rpg, ldg = x.numel() // C_, 1, 0
-    if gate is not None:
-        ldg = _rows_of(gate, "gate", C_, x.device, branch_dtype)
-        gates = gate.numel() // C_
-        if (rows % gates if gates else rows) != 0:
-            raise ValueError(f"gate: {gates} rows do not divide the {rows} rows of the stream")
-        rpg = rows // gates if gates and rows else 1
-    d = _ResidualNormDesc(rows=rows, rows_per_gate=rpg, ldg=ldg, channels=C_, stream_type=_type_of(x, "stream"),
-                          branch_type=_types()[branch_dtype], kind=_KINDS[kind], norms=_NORMS[norms], gate_act=_GATES[gate_act],
-                          scale=scale, eps=eps)
-    return d, rows, C_, x.device
+    return shape, x.numel() // shape[-1], dev, code, _NORMS[norms]
+
+
+def _empty(like, shape, ld):
+    # empty_like is the cheaper call, but keeps the order of dimensions
+    return _torch.empty_like(like) if ld == shape[-1] else like.new_empty(shape)
+
+
+def _gate_rows(gate, shape, rows, dtype, dev):
+    """(rows that share a gate row, its pitch)"""
+    C_ = shape[-1]
+    if gate.dim() == 0 or gate.shape[-1] != C_:
+        raise ValueError(f"gate: expected {C_} channels in the last dimension, got shape {tuple(gate.shape)}")
+    gates = gate.numel() // C_
+    if (rows % gates if gates else rows) != 0:
+        raise ValueError(f"gate: {gates} rows do not divide the {rows} rows of the stream")
+    return rows // gates if rows else 1, _pitch(gate, "gate", gate.shape, dtype, dev)
 
 
 def residual_norm(x, y=None, gate=None, post_gain=None, post_bias=None, pre_gain=None, pre_bias=None, norms="both", kind="rms",
@@ -975,29 +983,42 @@ def residual_norm(x, y=None, gate=None, post_gain=None, post_bias=None, pre_gain
     the channels of each image of an NHWC batch.  norms 'both', 'post' or 'pre', kind 'rms' or 'layer', gains and biases float32.
     Without y: n = pre(x) in branch_dtype (default x's), and h is x.  h, n: tensors to write (h may be x, n may be y), default new
     ones.  Returns (h, n), n None with norms 'post'.  Runs on `stream` (a hipStream_t as int), default torch's current one."""
-    tt = _types()
+    if stream is not None:
+        with _on(stream, x.device):
+            return residual_norm(x, y, gate, post_gain, post_bias, pre_gain, pre_bias, norms, kind, gate_act, scale, eps, branch_dtype, h, n)
+    shape, rows, dev, st, mask = _block(x, norms, kind, gate_act)
+    C_ = shape[-1]
     bt = y.dtype if y is not None else branch_dtype or x.dtype
-    if bt not in tt:
-        raise ValueError(f"y: float32, bfloat16 or float16, got {bt}")
-    if y is None and (norms != "pre" or gate is not None or h is not None):
-        raise ValueError("without y there is only norms='pre', and neither gate nor h")
-    d, rows, C_, dev = _block(x, bt, gate, norms, kind, gate_act, scale, eps)
-    d.ldx = _rows_of(x, "x", C_, dev)
+    rpg, ldg, ldy, ldh, ldn = 1, 0, 0, 0, 0
+    ldx = _pitch(x, "x", shape, x.dtype, dev)
     if y is not None:
-        d.ldy = _rows_of(y, "y", C_, dev, bt, rows)
+        ldy = _pitch(y, "y", shape, bt, dev)
+        if gate is not None:
+            rpg, ldg = _gate_rows(gate, shape, rows, bt, dev)
         if h is None:
-            h = _torch.empty(x.shape, dtype=x.dtype, device=dev)
-        d.ldh = _rows_of(h, "h", C_, dev, x.dtype, rows)
-    if norms == "post":
-        if n is not None:
-            raise ValueError("norms='post' has no n")
-    else:
+            h = _empty(x, shape, ldx)
+            ldh = C_
+        else:
+            ldh = _pitch(h, "h", shape, x.dtype, dev)
+    elif mask != 2 or gate is not None or h is not None:
+        raise ValueError("without y there is only norms='pre', and neither gate nor h")
+    if mask & 2:
         if n is None:
-            n = _torch.empty(x.shape, dtype=bt, device=dev)
-        d.ldn = _rows_of(n, "n", C_, dev, bt, rows)
-    _check(lib().sr_op_residual_norm(dev.index, C.byref(d), x.data_ptr(), _at(y), _at(gate), _vector(post_gain, "post_gain", C_, dev),
-                                     _vector(post_bias, "post_bias", C_, dev), _vector(pre_gain, "pre_gain", C_, dev),
-                                     _vector(pre_bias, "pre_bias", C_, dev), _at(h), _at(n), _stream_of(stream, dev)))
+            n = _empty(y, shape, ldy) if y is not None else _torch.empty(shape, dtype=bt, device=x.device)
+            ldn = C_
+        else:
+            ldn = _pitch(n, "n", shape, bt, dev)
+    elif n is not None:
+        raise ValueError("norms='post' has no n")
+    d = _pack_block(rows, rpg, ldx, ldy, ldg, ldh, ldn, 0, 0, 0, 0, 0, C_, st, _type_of(bt, "y"), _KINDS[kind], mask, _GATES[gate_act],
+                    scale, eps)
+    rc = lib().sr_op_residual_norm(dev, d, x.data_ptr(), None if y is None else y.data_ptr(), None if gate is None else gate.data_ptr(),
+                                   _vector(post_gain, "post_gain", C_, dev), _vector(post_bias, "post_bias", C_, dev),
+                                   _vector(pre_gain, "pre_gain", C_, dev), _vector(pre_bias, "pre_bias", C_, dev),
+                                   None if h is None else h.data_ptr(), None if n is None else n.data_ptr(),
+                                   _current_stream(dev))
+    if rc:
+        _check(rc)
     return (x if y is None else h), n
 
 
@@ -1012,78 +1033,103 @@ def residual_norm_bwd(h, y=None, dh=None, dn=None, gate=None, post_gain=None, po
     dgate (None without gate), and of the norms that are there the gains' and, with bias_grads, the biases' gradients (float32; of
     every norm that is there, whether or not its gain is given).  branch False: the forward call had no y; then only dx and the
     pre norm's vectors.  dx, dy: tensors to write, default new ones (dx may be dh, dy may be y or dn)."""
-    tt = _types()
-    post, pre = norms in ("post", "both"), norms in ("pre", "both")
+    if stream is not None:
+        with _on(stream, h.device):
+            return residual_norm_bwd(h, y, dh, dn, gate, post_gain, post_bias, pre_gain, norms, kind, gate_act, scale, eps, bias_grads, branch,
+                                     dx, dy)
+    shape, rows, dev, st, mask = _block(h, norms, kind, gate_act)
+    C_ = shape[-1]
+    post, pre = mask & 1, mask & 2
     if branch is None:
-        branch = post or y is not None
+        branch = bool(post) or y is not None
     if (pre and dn is None) or (not pre and dh is None):
         raise ValueError("dn is needed with the pre norm, dh without it")
     if (post or gate is not None) and (y is None or not branch):
         raise ValueError("y is needed with the post norm or a gate")
-    like = y if y is not None else dn if dn is not None else h
-    bt = like.dtype
-    if bt not in tt:
-        raise ValueError(f"y: float32, bfloat16 or float16, got {bt}")
-    d, rows, C_, dev = _block(h, bt, gate, norms, kind, gate_act, scale, eps)
-    d.ldh = _rows_of(h, "h", C_, dev)
-    if y is not None:
-        d.ldy = _rows_of(y, "y", C_, dev, bt, rows)
-    if dh is not None:
-        d.lddh = _rows_of(dh, "dh", C_, dev, h.dtype, rows)
-    if pre:
-        d.lddn = _rows_of(dn, "dn", C_, dev, bt, rows)
-    else:
+    if not pre:
         dn = None
+    like = y if y is not None else dn
+    bt = like.dtype
+    rpg, ldy, ldg, lddh, lddn = 1, 0, 0, 0, 0
+    ldh = _pitch(h, "h", shape, h.dtype, dev)
+    if y is not None:
+        ldy = _pitch(y, "y", shape, bt, dev)
+    if gate is not None:
+        rpg, ldg = _gate_rows(gate, shape, rows, bt, dev)
+    if dh is not None:
+        lddh = _pitch(dh, "dh", shape, h.dtype, dev)
+    if dn is not None:
+        lddn = _pitch(dn, "dn", shape, bt, dev)
+    lddx = lddy = C_
     if dx is None:
-        dx = _torch.empty(h.shape, dtype=h.dtype, device=dev)
-    d.lddx = _rows_of(dx, "dx", C_, dev, h.dtype, rows)
+        dx = _empty(h, shape, ldh)
+    else:
+        lddx = _pitch(dx, "dx", shape, h.dtype, dev)
     if branch:
         if dy is None:
-            dy = _torch.empty(h.shape, dtype=bt, device=dev)
-        d.lddy = _rows_of(dy, "dy", C_, dev, bt, rows)
+            dy = _empty(like, shape, ldy if y is not None else lddn)
+        else:
+            lddy = _pitch(dy, "dy", shape, bt, dev)
     elif dy is not None:
         raise ValueError("dy without a branch")
-    dgate = None
-    if gate is not None:
-        dgate = _torch.empty(gate.shape, dtype=bt, device=dev)
-        d.lddg = C_
+    dgate = like.new_empty(gate.shape) if gate is not None else None
+    d = _pack_block(rows, rpg, 0, ldy, ldg, ldh, 0, lddh, lddn, lddx, lddy, C_, C_, st, _type_of(bt, "y"), _KINDS[kind], mask,
+                    _GATES[gate_act], scale, eps)
     need = C.c_size_t()
-    _check(lib().sr_op_residual_norm_bwd_workspace(C.byref(d), int(gate is not None), C.byref(need)))
-    ws = _torch.empty(need.value, dtype=_torch.uint8, device=dev)
-    vec = _torch.empty((4, C_), dtype=_torch.float32, device=dev)
-    want = (post, post and bias_grads, pre, pre and bias_grads)
-    out = [vec[i] if w else None for i, w in enumerate(want)]
-    base = vec.data_ptr()
-    _check(lib().sr_op_residual_norm_bwd(dev.index, C.byref(d), h.data_ptr(), _at(y), _at(gate), _vector(post_gain, "post_gain", C_, dev),
-                                         _vector(post_bias, "post_bias", C_, dev), _vector(pre_gain, "pre_gain", C_, dev), _at(dh), _at(dn),
-                                         dx.data_ptr(), _at(dy), _at(dgate), *[base + 4 * C_ * i if w else None for i, w in enumerate(want)],
-                                         ws.data_ptr(), need.value, _stream_of(stream, dev)))
+    rc = lib().sr_op_residual_norm_bwd_workspace(d, gate is not None, C.byref(need))
+    if rc:
+        _check(rc)
+    ws = _torch.empty(need.value, dtype=_torch.uint8, device=h.device)
+    out = [None] * 4
+    if bias_grads:
+        vec = _torch.empty((4 if mask == 3 else 2, C_), dtype=_torch.float32, device=h.device).unbind(0)
+        out[:2 if post else 0] = vec[:2 if post else 0]
+        if pre:
+            out[2:] = vec[-2:]
+    else:
+        vec = _torch.empty((2 if mask == 3 else 1, C_), dtype=_torch.float32, device=h.device).unbind(0)
+        if post:
+            out[0] = vec[0]
+        if pre:
+            out[2] = vec[-1]
+    rc = lib().sr_op_residual_norm_bwd(dev, d, h.data_ptr(), None if y is None else y.data_ptr(), None if gate is None else gate.data_ptr(),
+                                       _vector(post_gain, "post_gain", C_, dev), _vector(post_bias, "post_bias", C_, dev),
+                                       _vector(pre_gain, "pre_gain", C_, dev), None if dh is None else dh.data_ptr(),
+                                       None if dn is None else dn.data_ptr(), dx.data_ptr(), None if dy is None else dy.data_ptr(),
+                                       None if dgate is None else dgate.data_ptr(), *[None if v is None else v.data_ptr() for v in out],
+                                       ws.data_ptr(), need.value, _current_stream(dev))
+    if rc:
+        _check(rc)
     return ResidualNormGrads(dx, dy, dgate, *out)
 
 
 class TensorList:
     """Dense torch tensors on one GPU -- a model's gradients -- as grad_norm and clip_grads take them (include/sr_hip.h
     sr_tensors_create).  Any mix of float32, bfloat16 and float16, any sizes (0 too), any order of dimensions as long as the
-    elements leave no gaps.  Holds on to the tensors; a program whose gradients stay in the same buffers makes it once."""
+    elements leave no gaps.  Holds on to the tensors; a program whose gradients stay in the same buffers makes it once.  upload: leave
+    what the kernels need to know of the list on the GPU (sr_tensors_upload), not while a stream is captured."""
 
-    def __init__(self, tensors):
+    def __init__(self, tensors, upload=True):
         self.tensors = list(tensors)
         _types()
         self.device = self.tensors[0].device if self.tensors else _torch.device("cuda", _torch.cuda.current_device())
         if self.device.type != "cuda":
             raise ValueError(f"tensor 0 is on {self.device}: these operators have no CPU fallback")
+        self.index = self.device.index
         desc = (_TensorDesc * max(len(self.tensors), 1))()
         for i, t in enumerate(self.tensors):
             if t.device != self.device:
                 raise ValueError(f"tensor {i} is on {t.device}, tensor 0 on {self.device}")
             if not _dense(t):
                 raise ValueError(f"tensor {i} of shape {tuple(t.shape)} and strides {tuple(t.stride())} has gaps or repeats elements")
-            desc[i].data, desc[i].count, desc[i].type = t.data_ptr() or None, t.numel(), _type_of(t, f"tensor {i}")
+            desc[i].data, desc[i].count, desc[i].type = t.data_ptr() or None, t.numel(), _type_of(t.dtype, f"tensor {i}")
         self._h = _vp()
         _check(lib().sr_tensors_create(C.byref(self._h), self.device.index, len(self.tensors), desc))
         need = C.c_size_t()
         _check(lib().sr_tensors_workspace(self._h, C.byref(need)))
         self.workspace_bytes = need.value
+        if upload and not _torch.cuda.is_current_stream_capturing():
+            _check(lib().sr_tensors_upload(self._h))
 
     def __len__(self):
         return len(self.tensors)
@@ -1116,16 +1162,20 @@ def grad_norm(grads, scale=1.0, per_tensor=False, stream=None):
     """Global L2 norm of many gradients (a TensorList or a sequence of tensors), times scale, as a float32 tensor (1,) on their GPU:
     no synchronisation.  per_tensor: -> (norm, norms (n,)) with the norm of each.  include/sr_hip.h sr_op_grad_norm."""
     if not isinstance(grads, TensorList):
-        grads = TensorList(grads)
+        grads = TensorList(grads, upload=False)
     if not grads._h:
         raise ValueError("the TensorList is closed")
+    if stream is not None:
+        with _on(stream, grads.device):
+            return grad_norm(grads, scale, per_tensor)
     dev = grads.device
-    norm = _torch.empty(1, dtype=_torch.float32, device=dev)
-    each = _torch.empty(len(grads), dtype=_torch.float32, device=dev) if per_tensor else None
     ws = _torch.empty(grads.workspace_bytes, dtype=_torch.uint8, device=dev)
-    _check(lib().sr_op_grad_norm(grads._h, scale, norm.data_ptr(), each.data_ptr() or None if per_tensor else None, ws.data_ptr(),
-                                 grads.workspace_bytes, _stream_of(stream, dev)))
-    return (norm, each) if per_tensor else norm
+    norm, each = _torch.empty(1 + len(grads) if per_tensor else 1, dtype=_torch.float32, device=dev), None
+    if per_tensor:
+        norm, each = norm.split_with_sizes([1, len(grads)])
+    _check(lib().sr_op_grad_norm(grads._h, scale, norm.data_ptr(), None if each is None else norm.data_ptr() + 4, ws.data_ptr(),
+                                 grads.workspace_bytes, _current_stream(grads.index)))
+    return norm if each is None else (norm, each)
 
 
 def clip_grads(grads, max_norm, scale=1.0, out=None, stream=None):
@@ -1133,16 +1183,19 @@ def clip_grads(grads, max_norm, scale=1.0, out=None, stream=None):
     or into `out`, tensors of the same sizes and types.  grads, out: TensorLists or sequences of tensors.  Returns the norm before
     clipping (of the gradients times scale) as a float32 tensor (1,), without a synchronisation.  include/sr_hip.h sr_op_clip_grads."""
     if not isinstance(grads, TensorList):
-        grads = TensorList(grads)
+        grads = TensorList(grads, upload=False)
     if out is not None and not isinstance(out, TensorList):
-        out = TensorList(out)
+        out = TensorList(out, upload=False)
     if not grads._h or (out is not None and not out._h):
         raise ValueError("the TensorList is closed")
+    if stream is not None:
+        with _on(stream, grads.device):
+            return clip_grads(grads, max_norm, scale, out)
     dev = grads.device
     norm = _torch.empty(1, dtype=_torch.float32, device=dev)
     ws = _torch.empty(grads.workspace_bytes, dtype=_torch.uint8, device=dev)
     _check(lib().sr_op_clip_grads(grads._h, out._h if out is not None else None, max_norm, scale, norm.data_ptr(), ws.data_ptr(),
-                                  grads.workspace_bytes, _stream_of(stream, dev)))
+                                  grads.workspace_bytes, _current_stream(grads.index)))
     return norm
 
 

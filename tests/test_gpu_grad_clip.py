@@ -197,6 +197,33 @@ def test_captured_and_replayed(sh):
         assert torch.equal(sh.grad_norm(ts), norm)
 
 
+def test_long_list_captured_replayed_and_gone(sh):
+    """A graph does not read what the list has on the GPU: it is replayed after the list is gone and others took its place, one of
+    them while a capture is under way."""
+    ts = [randn(i, 1 + i * 13) for i in range(400)]
+    lst, out = sh.TensorList(ts), [torch.empty_like(t) for t in ts]
+    outs, old = sh.TensorList(out), sh.TensorList(ts[:200])
+    eager = sh.clip_grads(lst, 1.0, out=outs)
+    first = [o.clone() for o in out]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = sh.clip_grads(lst, 1.0, out=outs)
+        again = sh.grad_norm(ts)                 # a list made inside the capture
+        old.close()
+    del lst, outs
+    for i in range(3):
+        more = [sh.TensorList(ts[i:300 + i]) for i in range(4)]
+        for o in out:
+            o.fill_(0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(norm, eager) and torch.equal(again, eager)
+        for o, f in zip(out, first):
+            assert torch.equal(o, f)
+        del more
+
+
 def test_tensor_behind_2_31_elements(sh):
     t = torch.zeros((1 << 31) + 11, dtype=BF16, device="cuda")
     t[-1], t[1 << 30], t[0], t[(1 << 31)] = 2.0, 4.0, 4.0, 8.0

@@ -10,11 +10,18 @@ import sr_hip
 P = 1 << 20                    # addresses: 1 MiB apart
 
 
+class Desc(C.Structure):
+    _fields_ = ([("rows", C.c_int64), ("rows_per_gate", C.c_int64)]
+                + [(n, C.c_int64) for n in ("ldx", "ldy", "ldg", "ldh", "ldn", "lddh", "lddn", "lddx", "lddy", "lddg")]
+                + [(n, C.c_int32) for n in ("channels", "stream_type", "branch_type", "kind", "norms", "gate_act")]
+                + [("scale", C.c_float), ("eps", C.c_float)])
+
+
 def desc(**kw):
     d = dict(rows=4, rows_per_gate=1, channels=16, stream_type=0, branch_type=0, kind=0, norms=3, gate_act=0, scale=1.0, eps=1e-6)
     d.update({n: 16 for n in ("ldx", "ldy", "ldg", "ldh", "ldn", "lddh", "lddn", "lddx", "lddy", "lddg")})
     d.update(kw)
-    return sr_hip._ResidualNormDesc(**d)
+    return Desc(**d)
 
 
 def forward(d, x=P, y=2 * P, gate=None, pw=None, pb=None, qw=None, qb=None, h=3 * P, n=4 * P):
@@ -109,11 +116,11 @@ def test_tensor_lists():
     h = C.c_void_p()
     assert l.sr_tensors_create(C.byref(h), 0, -1, None) == -1 and l.sr_tensors_create(C.byref(h), 0, 2, None) == -1
     assert l.sr_tensors_create(C.byref(h), -1, 0, None) == -1
-    assert l.sr_tensors_destroy(None) == 0
+    assert l.sr_tensors_destroy(None) == 0 and l.sr_tensors_upload(None) == -1
     rc, h = tensors((None, 0, 0), (P, 100_000, 1), (2 * P, 3, 2))
     assert rc == 0
     need = C.c_size_t()
-    assert l.sr_tensors_workspace(h, C.byref(need)) == 0 and 8 * 14 <= need.value <= 8 * (2048 + 3)
+    assert l.sr_tensors_workspace(h, C.byref(need)) == 0 and 8 * 14 <= need.value <= 8 * (4096 + 3)
     W, N = 8 * P, 9 * P
     assert l.sr_op_grad_norm(h, 1.0, N, None, W, need.value, None) == -4              # as far as the device
     for args in ((None, 1.0, N, None, W, need.value, None), (h, 0.0, N, None, W, need.value, None), (h, 1.0, None, None, W, need.value, None),
@@ -121,7 +128,7 @@ def test_tensor_lists():
                  (h, 1.0, N, N, W, need.value, None), (h, 1.0, W + 8, None, W, need.value, None), (h, 1.0, P + 8, None, W, need.value, None),
                  (h, 1.0, N, W, W, need.value, None), (h, 1.0, N, None, P, need.value, None), (h, 1.0, N, 2 * P, W, need.value, None)):
         assert l.sr_op_grad_norm(*args) == -1, args
-    assert l.sr_op_clip_grads(h, None, 1.0, 1.0, N, W, need.value, None) == -4
+    assert l.sr_op_clip_grads(h, None, 1.0, 1.0, N, W, need.value, None) == -4 and l.sr_tensors_upload(h) == -4
     for m, s in ((0.0, 1.0), (-1.0, 1.0), (float("nan"), 1.0), (1.0, -1.0), (1.0, float("nan"))):
         assert l.sr_op_clip_grads(h, None, m, s, N, W, need.value, None) == -1
     for other in (((P, 100_000, 1), (2 * P, 3, 2)), ((None, 0, 0), (P, 99_999, 1), (2 * P, 3, 2)), ((None, 0, 0), (P, 100_000, 2), (2 * P, 3, 2)),
