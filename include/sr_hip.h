@@ -255,6 +255,15 @@ int sr_rccl_allreduce_f32(void* comm, float* d_buf, int64_t n, void* hip_stream)
 int sr_train_allreduce(sr_ctx* ctx, void* comm, float* d_grads);
 int sr_train_apply(sr_ctx* ctx, const float* d_grads, float grad_scale, float lr, float beta1,
                    float beta2, float eps);
+/* Gradient clipping of the optimizer steps, `clipnorm` of a Keras 2.2.4 optimizer (optimizers.py get_gradients: every gradient times
+ * clipnorm / norm where the global norm of all gradients of the model exceeds clipnorm).  0 (the state of a new ctx) = off; it holds
+ * for every later step of the ctx: sr_train_apply, sr_train_on_batch, sr_train_on_clips (the generator's gradient times grad_scale),
+ * sr_tecogan_apply and the combined steps of sr_tecogan_iteration (generator and, with train_disc, discriminator together).  The factor
+ * is applied inside the Adam update; the gradient vectors keep their values.  sr_train_grad_norm: the norm before clipping that the
+ * last step with clipping went by (synchronises; SR_ERR_STATE if there was none).  sr_disc_*: the same for sr_disc_apply and the
+ * discriminator's own steps of sr_tecogan_iteration. */
+int sr_train_set_clipnorm(sr_ctx* ctx, float clipnorm);
+int sr_train_grad_norm(sr_ctx* ctx, float* norm);
 int sr_train_on_batch(sr_ctx* ctx, int B, const float* lr_t, const float* lr_tm1, const float* est_tm1,
                       const float* hr_t, float lr, float* losses);
 int64_t sr_train_iterations(const sr_ctx* ctx);   /* optimizer steps taken (Keras `iterations`) */
@@ -323,6 +332,8 @@ int sr_disc_train_grads(sr_disc* d, int B, const float* const* imgs, const float
 int sr_disc_read_grads(sr_disc* d, float* out, int out_on_device);
 int sr_disc_apply(sr_disc* d, const float* d_grads, float grad_scale, float lr, float beta1, float beta2, float eps, int64_t t,
                   int slot, int reset_moments);
+int sr_disc_set_clipnorm(sr_disc* d, float clipnorm);
+int sr_disc_grad_norm(sr_disc* d, float* norm);
 /* tecogan.train_on_batch (reference TecoGAN.py:87-108,122-131,469-479) up to the optimizer, ctx model SR_TECOGAN:
  * inputs [lr_t, lr_tm1, est_tm1, next_est (I_hr_fut), next_hat_est (I_hr_warp_fut), bic_past, bic_pres, bic_fut], targets
  * [hr_t, ones, d_1..d_4 (d_targets: 4 host pointers), hr_t x 4 (VGG19 terms: evaluated when sr_tecogan_set_vgg attached the

@@ -63,9 +63,14 @@ class FrameRecurrentVideoSR(object):
         self.space2depth = Space2Depth(self.hr_shape, device=device).build()
         self.frvsr = GeneratorModel(self.core, 'FRVSR')
         # loss functions and learning rate of the reference (FRVSR.py:69-71)
-        self.opt = Adam(lr=1e-4)
+        self.opt = Adam(lr=1e-4, clipnorm=self._clipnorm())
         self.frvsr.compile(loss=['mean_squared_error', 'mean_squared_error'], loss_weights=[1., 1.], optimizer=self.opt)
         print('[INFO] Frame-Recurrent Video Super Resolution ready.')
+
+    def _clipnorm(self):
+        """train.clipnorm: the global gradient norm that the optimizer steps clip to (absent or 0: no clipping, the reference's way)."""
+        train = self.configs.get('train') if isinstance(self.configs, dict) else None
+        return (train or {}).get('clipnorm')
 
     # the model object holding the generator ('frvsr' here, 'generator' in TecoGAN)
     def _generator(self):

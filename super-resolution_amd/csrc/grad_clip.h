@@ -21,6 +21,10 @@ inline int64_t grad_chunks(uint32_t n, uint32_t chunk) { return ((int64_t)n + ch
 // parts[i] = sum of squares of chunk i; piece after piece, the chunks of a piece in order.  At most 160 pieces.
 hipError_t launch_grad_partials(const GradPiece* pieces, int n, uint32_t chunk, double* parts, hipStream_t s);
 
+// the same of one vector, however long; *nparts: how many partial sums there are (at most FLAT_PARTS)
+constexpr int FLAT_PARTS = GRAD_PARTS + 64;
+hipError_t launch_flat_partials(const float* g, int64_t n, double* parts, int* nparts, hipStream_t s);
+
 // What a kernel needs to know the norm of scaled gradients: two runs of partial sums (the second may be empty) and their scales
 struct ClipArgs {
     const double* parts;

@@ -193,6 +193,19 @@ hipError_t launch_grad_partials(const GradPiece* pieces, int n, uint32_t chunk, 
     return hipGetLastError();
 }
 
+hipError_t launch_flat_partials(const float* g, int64_t n, double* parts, int* nparts, hipStream_t s) {
+    GradPiece p[64];
+    const uint32_t chunk = grad_chunk(n);
+    int k = 0;
+    *nparts = 0;
+    for (int64_t at = 0; at < n; at += GRAD_PIECE, ++k) {
+        if (k == 64) return hipErrorInvalidValue;
+        p[k] = {g + at, (uint32_t)std::min<int64_t>(n - at, GRAD_PIECE), SR_T_F32};
+        *nparts += (int)grad_chunks(p[k].n, chunk);
+    }
+    return launch_grad_partials(p, k, chunk, parts, s);
+}
+
 }  // namespace sr
 
 // ------------------------------------------------------------------------------------------------- C ABI

@@ -226,6 +226,10 @@ hipError_t launch_mse_grad(const float* pred, const float* target, float* g, dou
                            int gcs, const float* clip_src, int tanh_out, hipStream_t s);
 hipError_t launch_adam(float* p, float* m, float* v, const float* g, long n, float lr_t, float b1, float b2, float eps,
                        float gscale, hipStream_t s);
+// the same update of a clipped gradient: g * gscale * clip_factor(c), the norm that `c` describes taken down to c.max_norm
+struct ClipArgs;
+hipError_t launch_adam_clip(float* p, float* m, float* v, const float* g, long n, float lr_t, float b1, float b2, float eps,
+                            float gscale, const ClipArgs& c, hipStream_t s);
 // ents: srh::PackEnt {int32 src, uint32 dst}[n]
 hipError_t launch_repack(const float* kernel, const void* ents, int n, void* out, int prec, hipStream_t s);
 // batched form: job q re-packs params[src + ents[i].src] into out (ents == nullptr: copies n floats, a bias)

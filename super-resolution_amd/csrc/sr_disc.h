@@ -25,6 +25,9 @@ struct sr_disc {
     float *wg_part = nullptr, *dw3 = nullptr;
     float* in9[9] = {};                    // device copies of the nine input images (host entry points)
     float* featT[4] = {};                  // device copies of feature-map targets
+    float clipnorm = 0.f;                  // sr_disc_set_clipnorm; 0: off
+    double* clip_parts = nullptr;          // partial sums of a clipped step, the norm behind them (allocated by the first one)
+    bool clipped = false;                  // there was one
     std::vector<float*> it_buf;            // sr_tecogan_iteration: the thirteen HR arrays of one pass (allocated on first use)
 };
 
@@ -41,8 +44,9 @@ int disc_forward(sr_disc* d, int B, const sr::Ptr9& imgs, bool training, bool up
 // losses land in d->d_loss[1..4]; want_wgrads: parameter gradients into d->d_grad; want_dx: d->gS = gradient of the 27
 // (32) input channels [B,H,W,32]
 int disc_backward(sr_disc* d, int B, const float* const* feat_targets, const float* feat_w, bool want_wgrads, bool want_dx);
-// Adam (Keras 2.2.4) on the trainable tensors with moment slot `slot`, then re-pack of the conv weights
+// Adam (Keras 2.2.4) on the trainable tensors with moment slot `slot`, then re-pack of the conv weights.  clip: the norm a combined
+// step goes by (nullptr: that step does not clip); without `combined` the object's own clipnorm decides
 int disc_apply(sr_disc* d, const float* d_grads, float grad_scale, float lr, float beta1, float beta2, float eps, int64_t t, int slot,
-               bool reset_moments);
+               bool reset_moments, bool combined = false, const sr::ClipArgs* clip = nullptr);
 
 }  // namespace srh

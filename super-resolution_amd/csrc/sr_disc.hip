@@ -9,6 +9,7 @@
 // tap x phase cells are used).  Forward, data gradient (+ depth_to_space) and weight gradient (+ gather) all reuse
 // conv3x3_lds_kernel / wgrad_kernel; the price is 2.25x the layer's MACs, bought back by not writing a second
 // conv family for a model that is 1/3 of the adversarial step.
+#include "grad_clip.h"
 #include "sr_disc.h"
 
 #include <cmath>
@@ -218,7 +219,7 @@ int disc_backward(sr_disc* d, int B, const float* const* feat_targets, const flo
 }
 
 int disc_apply(sr_disc* d, const float* d_grads, float grad_scale, float lr, float beta1, float beta2, float eps, int64_t t, int slot,
-               bool reset_moments) {
+               bool reset_moments, bool combined, const ClipArgs* clip) {
     if (slot < 0 || slot > 1) return dfail(d, SR_ERR_ARG, "Adam slot must be 0 (discriminator) or 1 (tecogan)");
     if (t < 1) return dfail(d, SR_ERR_ARG, "Adam iteration must be >= 1");
     hipStream_t st = d->stream;
@@ -229,8 +230,19 @@ int disc_apply(sr_disc* d, const float* d_grads, float grad_scale, float lr, flo
     }
     const double lr_t = (double)lr * std::sqrt(1.0 - std::pow((double)beta2, (double)t)) / (1.0 - std::pow((double)beta1, (double)t));
     // the gradient entries of the moving statistics are zero and never written: Adam leaves them alone
-    DCHK(d, launch_adam(d->d_params, d->d_m[slot], d->d_v[slot], d_grads ? d_grads : d->d_grad, d->nparams, (float)lr_t, beta1, beta2, eps,
-                        grad_scale, st));
+    const float* g = d_grads ? d_grads : d->d_grad;
+    ClipArgs own;
+    if (!combined && d->clipnorm > 0.f) {
+        if (!d->clip_parts) DCHK(d, hipMalloc((void**)&d->clip_parts, (FLAT_PARTS + 1) * sizeof(double)));
+        own = {d->clip_parts, 0, 0, grad_scale, 0.f, d->clipnorm, (float*)(d->clip_parts + FLAT_PARTS)};
+        DCHK(d, launch_flat_partials(g, d->nparams, d->clip_parts, &own.n0, st));
+        d->clipped = true;
+        clip = &own;
+    }
+    if (clip)
+        DCHK(d, launch_adam_clip(d->d_params, d->d_m[slot], d->d_v[slot], g, d->nparams, (float)lr_t, beta1, beta2, eps, grad_scale, *clip, st));
+    else
+        DCHK(d, launch_adam(d->d_params, d->d_m[slot], d->d_v[slot], g, d->nparams, (float)lr_t, beta1, beta2, eps, grad_scale, st));
     d->host_stale = true;
     return disc_repack(d);
 }
@@ -261,6 +273,7 @@ int sr_disc_destroy(sr_disc* d) {
     for (float* p : d->it_buf)
         if (p) (void)hipFree(p);
     if (d->red) (void)hipFree(d->red);
+    if (d->clip_parts) (void)hipFree(d->clip_parts);
     for (int l = 0; l < 5; ++l) {
         free_layer(d->conv[l]);
         free_layer(d->conv_dg[l]);
@@ -482,6 +495,22 @@ int sr_disc_apply(sr_disc* d, const float* d_grads, float grad_scale, float lr, 
     if (!d->committed) return dfail(d, SR_ERR_WEIGHTS, "weights not committed");
     DCHK(d, hipSetDevice(d->device));
     return disc_apply(d, d_grads, grad_scale, lr, beta1, beta2, eps, t, slot, reset_moments != 0);
+}
+
+int sr_disc_set_clipnorm(sr_disc* d, float clipnorm) {
+    if (!d) return dfail(nullptr, SR_ERR_ARG, "discriminator is NULL");
+    if (!(clipnorm >= 0.f && clipnorm < 3e38f)) return dfail(d, SR_ERR_ARG, "clipnorm must be 0 (off) or positive and finite");
+    d->clipnorm = clipnorm;
+    return SR_OK;
+}
+
+int sr_disc_grad_norm(sr_disc* d, float* norm) {
+    if (!d || !norm) return dfail(d, SR_ERR_ARG, "NULL argument");
+    if (!d->clipped) return dfail(d, SR_ERR_STATE, "no step with clipping yet");
+    DCHK(d, hipSetDevice(d->device));
+    DCHK(d, hipStreamSynchronize(d->stream));
+    DCHK(d, hipMemcpy(norm, d->clip_parts + FLAT_PARTS, 4, hipMemcpyDeviceToHost));
+    return SR_OK;
 }
 
 int sr_disc_sync(sr_disc* d) {

@@ -148,6 +148,7 @@ struct sr_ctx {
     std::vector<hipEvent_t> ev_pool;
     // training (sr_train.hip); the host copies in `tensors` are stale while train->host_stale
     sr_train_state* train = nullptr;
+    float clipnorm = 0.f;    // sr_train_set_clipnorm; 0: off
     sr_vgg* vgg = nullptr;   // VGG19 feature terms of the combined step (sr_tecogan_set_vgg); not owned
 };
 

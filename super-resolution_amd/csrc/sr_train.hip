@@ -13,6 +13,7 @@
 #include <condition_variable>
 #include <mutex>
 #include <thread>
+#include "grad_clip.h"
 #include "sr_disc.h"
 #include "sr_vgg.h"
 
@@ -28,6 +29,8 @@ struct sr_train_state {
     float *d_params = nullptr, *d_m = nullptr, *d_v = nullptr, *d_grad = nullptr;
     int64_t t = 0;                      // optimizer iterations
     float *d_m2 = nullptr, *d_v2 = nullptr;   // Adam moments of the generator inside tecogan.train_on_batch (its own train function)
+    double* clip_parts = nullptr;       // partial sums of a clipped step (two vectors), the norm behind them; allocated by the first one
+    bool clipped = false;               // there was one
     bool host_stale = false;            // ctx->tensors older than d_params
     ConvLayer fnet_dg[14], srnet_dg[24];   // data-gradient convs of the Conv2D layers (planned where needed)
     std::map<std::string, float*> act;  // saved activations and gradient work buffers
@@ -629,6 +632,18 @@ int grads_common(sr_ctx* c, int B, const float* lr_t, const float* lr_tm1, const
     return finish_losses(c, losses);
 }
 
+// What the Adam step of a ctx with clipnorm goes by: the partial sums of the generator's gradient and, in a combined step, of the
+// discriminator's, enqueued here
+int clip_norm(sr_ctx* c, const float* g, float scale, const float* gd, int64_t nd, float scale_d, ClipArgs* a) {
+    sr_train_state* T = c->train;
+    if (!T->clip_parts) HIPCHK(c, hipMalloc((void**)&T->clip_parts, (2 * FLAT_PARTS + 1) * sizeof(double)));
+    *a = {T->clip_parts, 0, 0, scale, scale_d, c->clipnorm, (float*)(T->clip_parts + 2 * FLAT_PARTS)};
+    LAUNCHCHK(c, "grad norm", launch_flat_partials(g, T->nparams, T->clip_parts, &a->n0, c->stream));
+    if (gd) LAUNCHCHK(c, "grad norm", launch_flat_partials(gd, nd, T->clip_parts + a->n0, &a->n1, c->stream));
+    T->clipped = true;
+    return SR_OK;
+}
+
 // packed MFMA buffers of every conv (forward, data gradient, fused tap projection) from the master weights
 int repack_all(sr_ctx* c) {
     sr_train_state* T = c->train;
@@ -677,6 +692,7 @@ void train_free(sr_ctx* c) {
     for (auto p : fl)
         if (p) (void)hipFree(p);
     if (T->mse_part) (void)hipFree(T->mse_part);
+    if (T->clip_parts) (void)hipFree(T->clip_parts);
     for (void* p : {(void*)T->clip_lr, (void*)T->clip_est, (void*)T->clip_u8})
         if (p) (void)hipFree(p);
     for (hipStream_t cs : T->copy_stream)
@@ -764,11 +780,33 @@ int sr_train_apply(sr_ctx* c, const float* d_grads, float grad_scale, float lr, 
     T->t += 1;
     // Keras 2.2.4 Adam.get_updates: lr_t = lr * sqrt(1 - beta_2^t) / (1 - beta_1^t)
     const double lr_t = (double)lr * std::sqrt(1.0 - std::pow((double)beta2, (double)T->t)) / (1.0 - std::pow((double)beta1, (double)T->t));
-    LAUNCHCHK(c, "adam", launch_adam(T->d_params, T->d_m, T->d_v, d_grads ? d_grads : T->d_grad, T->nparams, (float)lr_t, beta1,
-                                     beta2, eps, grad_scale, c->stream));
+    const float* g = d_grads ? d_grads : T->d_grad;
+    if (c->clipnorm > 0.f) {
+        ClipArgs clip;
+        RC(clip_norm(c, g, grad_scale, nullptr, 0, 0.f, &clip));
+        LAUNCHCHK(c, "adam", launch_adam_clip(T->d_params, T->d_m, T->d_v, g, T->nparams, (float)lr_t, beta1, beta2, eps, grad_scale, clip, c->stream));
+    } else {
+        LAUNCHCHK(c, "adam", launch_adam(T->d_params, T->d_m, T->d_v, g, T->nparams, (float)lr_t, beta1, beta2, eps, grad_scale, c->stream));
+    }
     T->host_stale = true;
     c->mx6_valid = false;   // SR_F16MX6: the host-packed conv_trunk6.hip weights are stale; steps run on the bf16x3 kernels
     return repack_all(c);
+}
+
+int sr_train_set_clipnorm(sr_ctx* c, float clipnorm) {
+    if (!c) return fail(nullptr, SR_ERR_ARG, "ctx is NULL");
+    if (!(clipnorm >= 0.f && clipnorm < 3e38f)) return fail(c, SR_ERR_ARG, "clipnorm must be 0 (off) or positive and finite");
+    c->clipnorm = clipnorm;
+    return SR_OK;
+}
+
+int sr_train_grad_norm(sr_ctx* c, float* norm) {
+    if (!c || !norm) return fail(c, SR_ERR_ARG, "NULL argument");
+    if (!c->train || !c->train->clipped) return fail(c, SR_ERR_STATE, "no step with clipping yet");
+    HIPCHK(c, hipSetDevice(c->device));
+    HIPCHK(c, hipStreamSynchronize(c->stream));
+    HIPCHK(c, hipMemcpy(norm, c->train->clip_parts + 2 * FLAT_PARTS, 4, hipMemcpyDeviceToHost));
+    return SR_OK;
 }
 
 int sr_train_on_batch(sr_ctx* c, int B, const float* lr_t, const float* lr_tm1, const float* est_tm1, const float* hr_t,
@@ -1219,8 +1257,17 @@ static int tecogan_adam(sr_ctx* c, sr_disc* d, const float* d_gen_grads, const f
         HIPCHK(c, hipMemsetAsync(T->d_v2, 0, nb, c->stream));
     }
     const double lr_t = (double)lr * std::sqrt(1.0 - std::pow((double)beta2, (double)t)) / (1.0 - std::pow((double)beta1, (double)t));
-    LAUNCHCHK(c, "adam", launch_adam(T->d_params, T->d_m2, T->d_v2, d_gen_grads ? d_gen_grads : T->d_grad, T->nparams, (float)lr_t, beta1,
-                                     beta2, eps, d_gen_grads ? grad_scale : 1.f, c->stream));
+    const float *g = d_gen_grads ? d_gen_grads : T->d_grad, *gd = d_disc_grads ? d_disc_grads : d->d_grad;
+    const float scale = d_gen_grads ? grad_scale : 1.f, scale_d = d_disc_grads ? grad_scale : 1.f;
+    const bool clipping = c->clipnorm > 0.f;
+    ClipArgs clip;
+    if (clipping) {
+        if (train_disc) HIPCHK(c, hipStreamSynchronize(d->stream));      // whatever wrote the discriminator's gradient there
+        RC(clip_norm(c, g, scale, train_disc ? gd : nullptr, d->nparams, scale_d, &clip));
+        LAUNCHCHK(c, "adam", launch_adam_clip(T->d_params, T->d_m2, T->d_v2, g, T->nparams, (float)lr_t, beta1, beta2, eps, scale, clip, c->stream));
+    } else {
+        LAUNCHCHK(c, "adam", launch_adam(T->d_params, T->d_m2, T->d_v2, g, T->nparams, (float)lr_t, beta1, beta2, eps, scale, c->stream));
+    }
     T->host_stale = true;
     c->mx6_valid = false;
     int rc = repack_all(c);
@@ -1228,7 +1275,7 @@ static int tecogan_adam(sr_ctx* c, sr_disc* d, const float* d_gen_grads, const f
     if (train_disc) {
         HIPCHK(c, hipStreamSynchronize(c->stream));
         HIPCHK(c, hipStreamSynchronize(d->stream));
-        if ((rc = disc_apply(d, d_disc_grads, d_disc_grads ? grad_scale : 1.f, lr, beta1, beta2, eps, t, 1, false)))
+        if ((rc = disc_apply(d, d_disc_grads, scale_d, lr, beta1, beta2, eps, t, 1, false, true, clipping ? &clip : nullptr)))
             return fail(c, rc, "%s", d->err.c_str());
     }
     return SR_OK;

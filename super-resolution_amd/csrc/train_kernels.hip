@@ -24,6 +24,7 @@
 //   adam, repack  optimizer update on the flat parameter vector and the re-pack of the updated
 //                 kernels into the MFMA fragment order of the forward / dgrad convolutions (repack_batch:
 //                 every buffer of the network in two launches, job table in the kernel arguments).
+#include "grad_clip.h"
 #include "kernels.h"
 #include "gather_math.h"
 
@@ -1037,16 +1038,39 @@ hipError_t launch_mse_grad(const float* pred, const float* target, float* g, dou
 }
 
 // ================================================================== Adam (Keras 2.2.4 optimizers.py) and re-pack
-__global__ void adam_kernel(float* __restrict__ p, float* __restrict__ m, float* __restrict__ v, const float* __restrict__ g,
-                            long n, float lr_t, float b1, float b2, float eps, float gscale) {
-    const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= n) return;
+__device__ __forceinline__ void adam_update(float* __restrict__ p, float* __restrict__ m, float* __restrict__ v,
+                                            const float* __restrict__ g, long i, float lr_t, float b1, float b2, float eps, float gscale) {
     const float gi = g[i] * gscale;
     const float mi = b1 * m[i] + (1.f - b1) * gi;
     const float vi = b2 * v[i] + (1.f - b2) * gi * gi;
     m[i] = mi;
     v[i] = vi;
     p[i] -= lr_t * mi / (sqrtf(vi) + eps);
+}
+
+__global__ void adam_kernel(float* __restrict__ p, float* __restrict__ m, float* __restrict__ v, const float* __restrict__ g,
+                            long n, float lr_t, float b1, float b2, float eps, float gscale) {
+    const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= n) return;
+    adam_update(p, m, v, g, i, lr_t, b1, b2, eps, gscale);
+}
+
+// Keras 2.2.4 `clipnorm` (optimizers.py get_gradients: all gradients scaled by clipnorm / norm where their global norm reaches
+// it) inside the update: each workgroup derives the factor from the partial sums, the gradient is not written again.  1024
+// workgroups walk the vector, so that the partial sums (8 KB or less for these networks) are added 1024 times and not 10,000.
+__global__ void __launch_bounds__(256) adam_clip_kernel(float* __restrict__ p, float* __restrict__ m, float* __restrict__ v,
+                                                        const float* __restrict__ g, long n, float lr_t, float b1, float b2, float eps,
+                                                        float gscale, const ClipArgs c) {
+    __shared__ double lds4[4];
+    const float gs = gscale * clip_factor(c, lds4);
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) adam_update(p, m, v, g, i, lr_t, b1, b2, eps, gs);
+}
+
+hipError_t launch_adam_clip(float* p, float* m, float* v, const float* g, long n, float lr_t, float b1, float b2, float eps,
+                            float gscale, const ClipArgs& c, hipStream_t s) {
+    const int blocks = blocks_for(n, 256);
+    hipLaunchKernelGGL(adam_clip_kernel, dim3(blocks < 1024 ? blocks : 1024), dim3(256), 0, s, p, m, v, g, n, lr_t, b1, b2, eps, gscale, c);
+    return hipGetLastError();
 }
 
 hipError_t launch_adam(float* p, float* m, float* v, const float* g, long n, float lr_t, float b1, float b2, float eps,

@@ -298,13 +298,18 @@ class Warp(object):
 
 class Adam(object):
     """keras.optimizers.Adam as the reference constructs it (FRVSR.py:69: ``Adam(lr=1e-4)``); Keras 2.2.4
-    defaults for the rest.  The update itself runs on the device (sr_train_apply)."""
+    defaults for the rest.  The update itself runs on the device (sr_train_apply).  clipnorm: the argument every Keras 2.2.4
+    optimizer takes -- where the global norm of a step's gradients (all of the model's trainable weights) exceeds it, they are
+    scaled down to it; 0 or None: no clipping."""
 
-    def __init__(self, lr=0.001, beta_1=0.9, beta_2=0.999, epsilon=None, decay=0., amsgrad=False):
+    def __init__(self, lr=0.001, beta_1=0.9, beta_2=0.999, epsilon=None, decay=0., amsgrad=False, clipnorm=None):
         if decay or amsgrad:
             raise NotImplementedError('Adam decay / amsgrad are not used by the reference and not built')
         self.lr, self.beta_1, self.beta_2 = float(lr), float(beta_1), float(beta_2)
         self.epsilon = 1e-7 if epsilon is None else float(epsilon)      # K.epsilon()
+        self.clipnorm = float(clipnorm or 0.)
+        if not 0. <= self.clipnorm < 3e38:
+            raise ValueError('clipnorm must be 0 (no clipping) or positive and finite, got %r' % (clipnorm,))
         # optimizer.iterations: ONE counter per Adam instance, shared by every model compiled with it (the reference
         # compiles generator, discriminator and tecogan with the same instance, TecoGAN.py:111-131); the moments belong
         # to each model's own train function
@@ -351,6 +356,7 @@ class GeneratorModel(_CoreModel):
             raise NotImplementedError('the second target must be I_LR_t (reference FRVSR.py:155)')
         ctx = self.core.ctx(len(lr_t))
         opt = self.optimizer
+        ctx.set_clipnorm(opt.clipnorm)
         import dp
         if dp.active():
             dp.init_if_needed()
@@ -377,6 +383,7 @@ class GeneratorModel(_CoreModel):
         hr_clips = np.asarray(hr_clips)
         ctx = self.core.ctx(hr_clips.shape[0] * hr_clips.shape[1])
         opt = self.optimizer
+        ctx.set_clipnorm(opt.clipnorm)
         import dp
         if dp.active():
             dp.init_if_needed()
@@ -554,6 +561,7 @@ class DiscriminatorModel(_Model):
         labels = np.asarray(_as_list(y)[0], np.float32).reshape(-1)
         d = self.native(len(imgs[0]))
         opt = self.optimizer
+        d.set_clipnorm(opt.clipnorm)
         opt.iterations += 1
         kw = dict(lr=opt.lr, beta_1=opt.beta_1, beta_2=opt.beta_2, epsilon=opt.epsilon, slot=0, reset_moments=self._fresh_moments)
         import dp
@@ -668,6 +676,7 @@ class TecoGANModel(_Model):
         d = self.disc.native(B)
         self.attach_vgg(ctx, B)
         opt = self.optimizer
+        ctx.set_clipnorm(opt.clipnorm)
         losses = sr_hip.tecogan_grads(ctx, d, lr_t, lr_tm1, est_tm1, next_est, next_hat_est, bic_past, bic_pres, bic_fut, y[0], y[2:6],
                                       y[10], self.loss_weights)
         opt.iterations += 1

@@ -76,6 +76,10 @@ SIGNATURES = {
     "sr_rccl_comm_destroy": (C.c_int, [_vp]),
     "sr_rccl_allreduce_f32": (C.c_int, [_vp, _vp, C.c_int64, _vp]),
     "sr_train_allreduce": (C.c_int, [_vp, _vp, _vp]),
+    "sr_train_set_clipnorm": (C.c_int, [_vp, C.c_float]),
+    "sr_train_grad_norm": (C.c_int, [_vp, _f32p]),
+    "sr_disc_set_clipnorm": (C.c_int, [_vp, C.c_float]),
+    "sr_disc_grad_norm": (C.c_int, [_vp, _f32p]),
     "sr_train_on_batch": (C.c_int, [_vp, C.c_int, _vp, _vp, _vp, _vp, C.c_float, _f32p]),
     "sr_train_iterations": (C.c_int64, [_vp]),
     "sr_train_clips_grads": (C.c_int, [_vp, C.c_int, C.c_int, _vp, C.c_int, _vp, _f32p]),
@@ -391,6 +395,17 @@ class Context:
     def train_apply(self, d_grads=None, grad_scale=1.0, lr=1e-4, beta_1=0.9, beta_2=0.999, epsilon=1e-7):
         _check(lib().sr_train_apply(self._h, _vp(d_grads) if d_grads else None, grad_scale, lr, beta_1, beta_2, epsilon), self._h)
 
+    def set_clipnorm(self, clipnorm):
+        """Global gradient norm that every later optimizer step of this context clips to; 0: off (include/sr_hip.h
+        sr_train_set_clipnorm)."""
+        _check(lib().sr_train_set_clipnorm(self._h, clipnorm), self._h)
+
+    def grad_norm(self):
+        """The gradient norm, before clipping, of the last step with clipping."""
+        v = C.c_float()
+        _check(lib().sr_train_grad_norm(self._h, C.byref(v)), self._h)
+        return v.value
+
     def train_on_batch(self, lr_t, lr_tm1, est_tm1, hr_t, lr=1e-4):
         B, a, b, c, d = self._train_inputs(lr_t, lr_tm1, est_tm1, hr_t)
         losses = (C.c_float * 3)()
@@ -566,6 +581,16 @@ class Discriminator:
         g = np.empty(self.param_count(), np.float32)
         self._check(lib().sr_disc_read_grads(self._h, _ptr(g), 0))
         return g
+
+    def set_clipnorm(self, clipnorm):
+        """As Context.set_clipnorm, for the discriminator's own steps (apply and those of tecogan_iteration)."""
+        self._check(lib().sr_disc_set_clipnorm(self._h, clipnorm))
+
+    def grad_norm(self):
+        """The gradient norm, before clipping, of the last such step with clipping."""
+        v = C.c_float()
+        self._check(lib().sr_disc_grad_norm(self._h, C.byref(v)))
+        return v.value
 
     def apply(self, t, d_grads=None, grad_scale=1.0, lr=5e-5, beta_1=0.9, beta_2=0.999, epsilon=1e-7, slot=0, reset_moments=False):
         self._check(lib().sr_disc_apply(self._h, _vp(d_grads) if d_grads else None, grad_scale, lr, beta_1, beta_2, epsilon, int(t),

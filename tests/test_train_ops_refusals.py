@@ -149,3 +149,15 @@ def test_python_side_needs_a_gpu():
         sr_hip.residual_norm(torch.zeros(2, 8), torch.zeros(2, 8))
     with pytest.raises(ValueError, match="no CPU fallback"):
         sr_hip.TensorList([torch.zeros(4)])
+
+
+def test_adam_clipnorm_argument():
+    from layers import Adam
+    assert Adam().clipnorm == 0.0 and Adam(clipnorm=None).clipnorm == 0.0 and Adam(clipnorm=2).clipnorm == 2.0
+    for bad in (-1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            Adam(clipnorm=bad)
+    l = sr_hip.lib()
+    v = C.c_float()
+    assert l.sr_train_set_clipnorm(None, 1.0) == -1 and l.sr_disc_set_clipnorm(None, 1.0) == -1
+    assert l.sr_train_grad_norm(None, C.byref(v)) == -1 and l.sr_disc_grad_norm(None, C.byref(v)) == -1
