@@ -56,8 +56,9 @@ struct BwdArgs {
     const void *h, *y, *gate, *dh, *dn;
     const float *pw, *pb, *qw;
     void *dx, *dy, *dgate;
-    float *part;                     // [blocks][nslot][C] partial sums of the gains' and biases' gradients
-    float *gpart;                    // [units][C] partial sums of dgate where a gate row spans several units
+    float *part;                     // [blocks][nslot][pitch] partial sums of the gains' and biases' gradients
+    float *gpart;                    // [units][pitch] partial sums of dgate where a gate row spans several units
+    int pitch;                       // C rounded up to 4: the sums are read 16 bytes at a time
     int ldh, ldy, ldg, lddh, lddn, lddx, lddy, lddg;
     Units u;
     int C, tl, flags;
@@ -564,7 +565,7 @@ __global__ void __launch_bounds__(BLK ? 1024 : 256, BLK ? 4 : 3) rn_bwd_kernel(c
             if (!BLK) __syncthreads();
             if (a.dgate) {
                 if (a.u.per_group == 1) leave(S_PB, sums, t, lds, row_of<TB>(a.dgate, group, a.lddg), false);
-                else leave(S_PB, sums, t, lds, a.gpart + (int64_t)u * a.C, false);
+                else leave(S_PB, sums, t, lds, a.gpart + (int64_t)u * a.pitch, false);
             }
             if (FULL) {
                 if (!BLK) __syncthreads();
@@ -572,70 +573,87 @@ __global__ void __launch_bounds__(BLK ? 1024 : 256, BLK ? 4 : 3) rn_bwd_kernel(c
             }
         }
         if (!BLK) __syncthreads();
-        float* part = a.part + (int64_t)blockIdx.x * a.nslot * a.C;
+        float* part = a.part + (int64_t)blockIdx.x * a.nslot * a.pitch;
         const bool add = u != blockIdx.x;
         if constexpr (BLK) {
-            if (a.slot[0] >= 0) leave(S_PW, sums, t, lds, part + (int64_t)a.slot[0] * a.C, add);
-            if (a.slot[2] >= 0) leave(S_QW, sums, t, lds, part + (int64_t)a.slot[2] * a.C, add);
-            if (FULL && a.slot[1] >= 0) leave(S_PB, sums, t, lds, part + (int64_t)a.slot[1] * a.C, add);
-            if (FULL && a.slot[3] >= 0) leave(S_QB, sums, t, lds, part + (int64_t)a.slot[3] * a.C, add);
+            if (a.slot[0] >= 0) leave(S_PW, sums, t, lds, part + (int64_t)a.slot[0] * a.pitch, add);
+            if (a.slot[2] >= 0) leave(S_QW, sums, t, lds, part + (int64_t)a.slot[2] * a.pitch, add);
+            if (FULL && a.slot[1] >= 0) leave(S_PB, sums, t, lds, part + (int64_t)a.slot[1] * a.pitch, add);
+            if (FULL && a.slot[3] >= 0) leave(S_QB, sums, t, lds, part + (int64_t)a.slot[3] * a.pitch, add);
         } else {                     // all columns of all sums at once: few columns would leave most threads idle
             for (int i = threadIdx.x; i < a.nslot * a.C; i += 256) {
                 const int slot = i / a.C, c = i - slot * a.C;
                 const int sum = slot == a.slot[0] ? S_PW : slot == a.slot[2] ? S_QW : slot == a.slot[1] ? S_PB : S_QB;
                 const float s = joined(sum, c, t, lds);
-                part[i] = add ? part[i] + s : s;
+                float* out = part + slot * a.pitch + c;
+                *out = add ? *out + s : s;
             }
             if (u + gridDim.x < a.u.units) __syncthreads();      // before the next unit's sums
         }
     }
 }
 
-// The partial sums of a backward pass joined in a fixed order: 16 columns x 64 slices a workgroup.  blockIdx.y < 4: the gradient
-// of that gain or bias over the workgroups; beyond: gate row blockIdx.y - 4 over its units.
+// The partial sums of a backward pass joined in a fixed order: 4 columns a thread, LC threads side by side, 1024 / LC slices of the
+// partial sums.  16 threads side by side read 256 bytes at a time (24 MB of sums for 6000 channels: 7.0 us, with 4 threads 12.9), 4
+// give four times the workgroups where the columns are few (2 x 771: 5.4 us instead of 12.4).  blockIdx.y < 4: the gradient of that gain or bias over the workgroups; beyond: gate row blockIdx.y - 4 over its
+// units.
 struct JoinArgs {
     const float* part;
     float* out[4];
-    int blocks, nslot, slot[4], C;
+    int blocks, nslot, slot[4], C, pitch;
     const float* gpart;
     void* dgate;
     int64_t lddg;
     int per_group, branch_type;
 };
 
+template <int LC>
 __global__ void __launch_bounds__(1024) rn_join_kernel(const JoinArgs a) {
-    __shared__ float sm[64][17];
-    const int cl = threadIdx.x & 15, sl = threadIdx.x >> 4, c = blockIdx.x * 16 + cl, job = blockIdx.y;
+    constexpr int SL = 1024 / LC;
+    __shared__ float4 sm[SL * LC];
+    const int cl = threadIdx.x % LC, sl = threadIdx.x / LC, c = (blockIdx.x * LC + cl) * 4, job = blockIdx.y;
     const bool gate = job >= 4;
     if (!gate && !a.out[job]) return;
-    const float* p = gate ? a.gpart + (int64_t)(job - 4) * a.per_group * a.C : a.part + (int64_t)a.slot[job] * a.C;
-    const int64_t step = gate ? a.C : (int64_t)a.nslot * a.C;
+    const float* p = gate ? a.gpart + (int64_t)(job - 4) * a.per_group * a.pitch : a.part + (int64_t)a.slot[job] * a.pitch;
+    const int64_t step = gate ? a.pitch : (int64_t)a.nslot * a.pitch;
     const int n = gate ? a.per_group : a.blocks;
-    float s = 0.f;
-    if (c < a.C) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < a.C) {                   // behind the last column is room, and what stands there stays unused
 #pragma unroll 8
-        for (int i = sl; i < n; i += 64) s += p[i * step + c];
+        for (int i = sl; i < n; i += SL) {
+            const float4 v = *reinterpret_cast<const float4*>(p + i * step + c);
+            s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
+        }
     }
-    sm[sl][cl] = s;
-    __syncthreads();
-    if (sl < 8) {
+    // the slices, eight to one each time
 #pragma unroll
-        for (int i = 1; i < 8; ++i) s += sm[sl + 8 * i][cl];
+    for (int h = SL; h > 1; h = (h + 7) / 8) {
+        const int next = (h + 7) / 8;
+        if (sl >= next && sl < h) sm[sl * LC + cl] = make_float4(s[0], s[1], s[2], s[3]);
+        __syncthreads();
+        if (sl < next) {
+#pragma unroll
+            for (int i = 1; i < 8; ++i) {
+                if (sl + i * next >= h) break;
+                const float4 o = sm[(sl + i * next) * LC + cl];
+                s[0] += o.x, s[1] += o.y, s[2] += o.z, s[3] += o.w;
+            }
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    if (sl < 8) sm[sl][cl] = s;
-    __syncthreads();
-    if (sl || c >= a.C) return;
+    if (sl) return;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += sm[i][cl];
-    if (!gate)
-        a.out[job][c] = s;
-    else if (a.branch_type == SR_T_F32)
-        ((float*)a.dgate)[(job - 4) * a.lddg + c] = s;
-    else if (a.branch_type == SR_T_BF16)
-        ((bf16_t*)a.dgate)[(job - 4) * a.lddg + c] = (bf16_t)s;
-    else
-        ((f16_t*)a.dgate)[(job - 4) * a.lddg + c] = (f16_t)s;
+    for (int k = 0; k < 4; ++k) {
+        if (c + k >= a.C) break;
+        if (!gate)
+            a.out[job][c + k] = s[k];
+        else if (a.branch_type == SR_T_F32)
+            ((float*)a.dgate)[(job - 4) * a.lddg + c + k] = s[k];
+        else if (a.branch_type == SR_T_BF16)
+            ((bf16_t*)a.dgate)[(job - 4) * a.lddg + c + k] = (bf16_t)s[k];
+        else
+            ((f16_t*)a.dgate)[(job - 4) * a.lddg + c + k] = (f16_t)s[k];
+    }
 }
 
 // ------------------------------------------------------------------------------------------------- host
@@ -741,8 +759,9 @@ BwdPlan bwd_plan(const sr_residual_norm_desc* d, bool gate, unsigned rpg, bool f
     const bool simple = !full && !gate && d->channels % 8 == 0;
     q.s = shape_of(d, d->channels <= WAVE_C || d->channels > 4096 || simple ? 8 : 4);
     q.p = split_of(d, q.s, gate, rpg, q.s.blk || simple ? 16 : 12);
-    q.part = round_up_sz((size_t)q.p.blocks * 4 * d->channels * 4);
-    q.bytes = q.part + (q.p.shared_gate && q.p.u.per_group > 1 ? (size_t)q.p.u.units * d->channels * 4 : 0);
+    const size_t row = (size_t)round_up(d->channels, 4) * 4;
+    q.part = round_up_sz((size_t)q.p.blocks * 4 * row);
+    q.bytes = q.part + (q.p.shared_gate && q.p.u.per_group > 1 ? (size_t)q.p.u.units * row : 0);
     return q;
 }
 
@@ -911,7 +930,7 @@ extern "C" int sr_op_residual_norm_bwd(int device, const sr_residual_norm_desc* 
     const Split& p = q.p;
     float* part = (float*)workspace;
     float* gpart = (float*)((char*)workspace + q.part);
-    JoinArgs j = {part, {}, p.blocks, 0, {-1, -1, -1, -1}, C, gpart, dgate, d->lddg, (int)p.u.per_group, d->branch_type};
+    JoinArgs j = {part, {}, p.blocks, 0, {-1, -1, -1, -1}, C, round_up(C, 4), gpart, dgate, d->lddg, (int)p.u.per_group, d->branch_type};
     for (int i = 0; i < 4; ++i) {
         j.out[i] = vec[i];
         if (vec[i]) j.slot[i] = j.nslot++;
@@ -920,7 +939,7 @@ extern "C" int sr_op_residual_norm_bwd(int device, const sr_residual_norm_desc* 
         const int flags = (dy ? F_BRANCH : 0) | (post ? F_POST : 0) | (pre ? F_PRE : 0) | (d->kind == SR_NORM_LAYER ? F_LAYER : 0) |
                           (d->gate_act == SR_GATE_SIGMOID ? F_SIGMOID : 0) | (dh ? F_STREAM_GRAD : 0) | (y ? F_READ_Y : 0);
         const BwdArgs a = {h, y, gate, dh, dn, post ? post_gain : nullptr, post ? post_bias : nullptr, pre ? pre_gain : nullptr, dx, dy, dgate,
-                           part, gpart, (int)d->ldh, (int)d->ldy, (int)d->ldg, (int)d->lddh, (int)d->lddn, (int)d->lddx, (int)d->lddy,
+                           part, gpart, j.pitch, (int)d->ldh, (int)d->ldy, (int)d->ldg, (int)d->lddh, (int)d->lddn, (int)d->lddx, (int)d->lddy,
                            (int)d->lddg, p.u, C, q.s.tl, flags, j.nslot, {j.slot[0], j.slot[1], j.slot[2], j.slot[3]}, d->scale, d->eps,
                            1.f / (float)C};
         const int gt = !gate ? G_NONE : p.shared_gate ? G_SHARED : G_ROW;
@@ -931,7 +950,10 @@ extern "C" int sr_op_residual_norm_bwd(int device, const sr_residual_norm_desc* 
     hipError_t e = hipGetLastError();
     const unsigned gates = dgate && p.shared_gate && p.u.per_group > 1 ? (unsigned)(d->rows / rpg) : 0;
     if (e == hipSuccess && (j.nslot || gates)) {
-        rn_join_kernel<<<dim3((C + 15) / 16, 4 + gates), 1024, 0, st>>>(j);
+        const bool wide = (int64_t)(j.nslot + gates) * C >= 2048;
+        const dim3 grid((C + (wide ? 63 : 15)) / (wide ? 64 : 16), 4 + gates);
+        if (wide) rn_join_kernel<16><<<grid, 1024, 0, st>>>(j);
+        else rn_join_kernel<4><<<grid, 1024, 0, st>>>(j);
         e = hipGetLastError();
     }
     if (e != hipSuccess) return fail(nullptr, SR_ERR_HIP, "launch residual_norm_bwd: %s", hipGetErrorString(e));
