@@ -123,9 +123,12 @@ __global__ void __launch_bounds__(256) grad_partials_kernel(const TABLE_T t, dou
 constexpr int EACH_MAX = 900;
 struct EachTable {
     uint32_t first[EACH_MAX + 1];   // partial sums of the tensors of this launch
-    int count;
 };
-__global__ void __launch_bounds__(256) grad_norm_kernel(const EachTable t, const double* __restrict__ parts, uint32_t nparts, float scale,
+struct EachRecords {
+    const uint32_t* first;
+};
+template <typename TABLE_T>
+__global__ void __launch_bounds__(256) grad_norm_kernel(const TABLE_T t, const double* __restrict__ parts, uint32_t nparts, float scale,
                                                         float* __restrict__ norm, float* __restrict__ each) {
     __shared__ double lds4[4];
     const int i = (int)blockIdx.x - 1;
@@ -217,7 +220,7 @@ struct sr_tensors {
     std::vector<std::pair<const char*, const char*>> sorted;   // byte ranges by address
     uint32_t chunk = 0;
     bool overlap = false;                    // two tensors share memory
-    Record* d_records = nullptr;             // of every chunk (sr_tensors_upload)
+    Record* d_records = nullptr;             // of every chunk (sr_tensors_upload), behind them `first`
 };
 
 #define GC_TRY(call)          \
@@ -249,8 +252,17 @@ void fill(Table& a, const sr_tensors* t, const sr_tensors* out, size_t at) {
     }
 }
 
-// Partial sums of the whole list, and with `c` the scaled gradients.  A captured call does not go by the list's own records: a graph
-// may outlive the list.
+// Does a call on `st` go by what sr_tensors_upload left of the lists?  A captured one does not: a graph may outlive the list.
+hipError_t uploaded(const sr_tensors* t, const sr_tensors* out, hipStream_t st, bool* yes) {
+    *yes = false;
+    if (!t->d_records || !out->d_records) return hipSuccess;
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    const hipError_t e = hipStreamIsCapturing(st, &capture);
+    *yes = capture == hipStreamCaptureStatusNone;
+    return e;
+}
+
+// Partial sums of the whole list, and with `c` the scaled gradients
 hipError_t launch_list(const sr_tensors* t, const sr_tensors* out, void* ws, const ClipArgs* c, hipStream_t st) {
     const uint32_t blocks = t->first.back();
     if (!blocks) return hipSuccess;
@@ -259,13 +271,11 @@ hipError_t launch_list(const sr_tensors* t, const sr_tensors* out, void* ws, con
         if (c) grad_scale_kernel<<<blocks, 256, 0, st>>>(table, *c);
         return hipGetLastError();
     };
+    bool have;
+    const hipError_t e = uploaded(t, out, st, &have);
+    if (e != hipSuccess) return e;
     Records r = {t->d_records, out->d_records};
-    if (r.src && r.dst) {
-        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-        const hipError_t e = hipStreamIsCapturing(st, &capture);
-        if (e != hipSuccess) return e;
-        if (capture == hipStreamCaptureStatusNone) return run(r);
-    }
+    if (have) return run(r);
     Table a;
     if (t->pieces.size() <= TABLE) {
         fill(a, t, out, 0);
@@ -376,8 +386,9 @@ int sr_tensors_upload(sr_tensors* t) {
                 r.push_back({(const char*)p.src + (size_t)at * type_bytes((int)type), std::min(t->chunk, all - at), type});
         }
         Record* d = nullptr;
-        HIPCHK(nullptr, hipMalloc((void**)&d, n * sizeof(Record)));
-        const hipError_t e = hipMemcpy(d, r.data(), n * sizeof(Record), hipMemcpyHostToDevice);
+        HIPCHK(nullptr, hipMalloc((void**)&d, n * sizeof(Record) + t->first.size() * 4));
+        hipError_t e = hipMemcpy(d, r.data(), n * sizeof(Record), hipMemcpyHostToDevice);
+        if (e == hipSuccess) e = hipMemcpy(d + n, t->first.data(), t->first.size() * 4, hipMemcpyHostToDevice);
         if (e != hipSuccess) {
             (void)hipFree(d);
             return fail(nullptr, SR_ERR_HIP, "%s: hipMemcpy failed: %s", who, hipGetErrorString(e));
@@ -420,14 +431,21 @@ int sr_op_grad_norm(const sr_tensors* t, float scale, float* d_norm, float* d_no
     hipStream_t st = (hipStream_t)hip_stream;
     double* parts = (double*)workspace;
     GC_TRY(launched(launch_list(t, t, workspace, nullptr, st), who));
+    bool have;
+    GC_TRY(launched(uploaded(t, t, st, &have), who));
+    if (have) {
+        const EachRecords e = {(const uint32_t*)(t->d_records + t->first.back())};
+        grad_norm_kernel<<<1 + (d_norms ? (int)n : 0), 256, 0, st>>>(e, parts, t->first.back(), scale, d_norm, d_norms);
+        return launched(hipGetLastError(), who);
+    }
     EachTable e;
     size_t at = 0;
     do {
-        e.count = d_norms ? (int)std::min<size_t>(n - at, EACH_MAX) : 0;
-        for (int i = 0; i <= e.count; ++i) e.first[i] = t->first[at + i];
-        grad_norm_kernel<<<1 + e.count, 256, 0, st>>>(e, parts, t->first.back(), scale, at ? nullptr : d_norm, d_norms + at);
+        const int count = d_norms ? (int)std::min<size_t>(n - at, EACH_MAX) : 0;
+        for (int i = 0; i <= count; ++i) e.first[i] = t->first[at + i];
+        grad_norm_kernel<<<1 + count, 256, 0, st>>>(e, parts, t->first.back(), scale, at ? nullptr : d_norm, d_norms + at);
         GC_TRY(launched(hipGetLastError(), who));
-        at += e.count;
+        at += count;
     } while (d_norms && at < n);
     return SR_OK;
 }

@@ -908,6 +908,7 @@ _GATES = {"linear": 0, "sigmoid": 1}
 _torch = None
 _torch_types = None
 _current_stream = None
+_bwd_bytes = {}      # bytes of workspace of the backward calls made so far
 # sr_residual_norm_desc: rows, rows_per_gate, ten pitches; channels, stream_type, branch_type, kind, norms, gate_act; scale, eps
 _pack_block = struct.Struct("=12q6i2f").pack
 
@@ -968,6 +969,10 @@ def _vector(t, what, C_, dev):
     if t.dtype is not _torch.float32 or t.get_device() != dev or t.dim() != 1 or t.numel() != C_ or not t.is_contiguous():
         raise ValueError(f"{what}: expected a contiguous float32 vector of {C_} on cuda:{dev}")
     return t.data_ptr()
+
+
+def _vector_like(gain, C_, h):
+    return _torch.empty_like(gain) if gain is not None else _torch.empty(C_, dtype=_torch.float32, device=h.device)
 
 
 def _block(x, norms, kind, gate_act):
@@ -1100,29 +1105,24 @@ def residual_norm_bwd(h, y=None, dh=None, dn=None, gate=None, post_gain=None, po
     dgate = like.new_empty(gate.shape) if gate is not None else None
     d = _pack_block(rows, rpg, 0, ldy, ldg, ldh, 0, lddh, lddn, lddx, lddy, C_, C_, st, _type_of(bt, "y"), _KINDS[kind], mask,
                     _GATES[gate_act], scale, eps)
-    need = C.c_size_t()
-    rc = lib().sr_op_residual_norm_bwd_workspace(d, gate is not None, C.byref(need))
-    if rc:
-        _check(rc)
-    ws = _torch.empty(need.value, dtype=_torch.uint8, device=h.device)
-    out = [None] * 4
-    if bias_grads:
-        vec = _torch.empty((4 if mask == 3 else 2, C_), dtype=_torch.float32, device=h.device).unbind(0)
-        out[:2 if post else 0] = vec[:2 if post else 0]
-        if pre:
-            out[2:] = vec[-2:]
-    else:
-        vec = _torch.empty((2 if mask == 3 else 1, C_), dtype=_torch.float32, device=h.device).unbind(0)
-        if post:
-            out[0] = vec[0]
-        if pre:
-            out[2] = vec[-1]
+    # the workspace goes by these alone
+    key = (rows, C_, st, bt, rpg, gate is None)
+    need = _bwd_bytes.get(key)
+    if need is None:
+        if len(_bwd_bytes) >= 4096:
+            _bwd_bytes.clear()
+        size = C.c_size_t()
+        _check(lib().sr_op_residual_norm_bwd_workspace(d, gate is not None, C.byref(size)))
+        need = _bwd_bytes[key] = size.value
+    ws = _torch.empty(need, dtype=_torch.uint8, device=h.device)
+    out = [_vector_like(post_gain, C_, h) if post else None, _vector_like(post_gain, C_, h) if post and bias_grads else None,
+           _vector_like(pre_gain, C_, h) if pre else None, _vector_like(pre_gain, C_, h) if pre and bias_grads else None]
     rc = lib().sr_op_residual_norm_bwd(dev, d, h.data_ptr(), None if y is None else y.data_ptr(), None if gate is None else gate.data_ptr(),
                                        _vector(post_gain, "post_gain", C_, dev), _vector(post_bias, "post_bias", C_, dev),
                                        _vector(pre_gain, "pre_gain", C_, dev), None if dh is None else dh.data_ptr(),
                                        None if dn is None else dn.data_ptr(), dx.data_ptr(), None if dy is None else dy.data_ptr(),
                                        None if dgate is None else dgate.data_ptr(), *[None if v is None else v.data_ptr() for v in out],
-                                       ws.data_ptr(), need.value, _current_stream(dev))
+                                       ws.data_ptr(), need, _current_stream(dev))
     if rc:
         _check(rc)
     return ResidualNormGrads(dx, dy, dgate, *out)
