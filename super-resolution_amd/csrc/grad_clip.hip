@@ -27,6 +27,12 @@ namespace {
 // the workspace, where a launch for every TABLE pieces (4.7 us each, mostly the way of the arguments) writes them first.  Clipping
 // 60 M elements in 700 tensors took 188 us with a launch for every 224 or 152 pieces.
 constexpr int TABLE = 160;
+// From 128 MB on, half of the last-level cache, clipped gradients are stored past the caches: their next reader would find the first
+// of them gone anyway, and the following pass over the gradients does not wait for them to be written back (60 M elements of three
+// types: 106 -> 84 us, 100 M bf16: 128 -> 106; 250 M bf16 at odd addresses: 315 -> 322; 5 M fp32 would gain 1 us and lose it to the
+// next reader).
+constexpr int64_t PAST_CACHES = 128 << 20;
+
 struct Piece {
     const void* src;
     void* dst;
@@ -141,7 +147,7 @@ __global__ void __launch_bounds__(256) grad_norm_kernel(const TABLE_T t, const d
     if (threadIdx.x == 0) *(i < 0 ? norm : each + i) = (float)(sqrt(s) * (double)scale);
 }
 
-template <typename T>
+template <bool NT, typename T>
 __device__ __forceinline__ void scale_run(const T* src, T* dst, uint32_t n, float f) {
     constexpr int V = 16 / sizeof(T);
     const uint32_t nv = n / V;
@@ -151,21 +157,22 @@ __device__ __forceinline__ void scale_run(const T* src, T* dst, uint32_t n, floa
         load_vec<T, V>(src + (size_t)i * V, v);
 #pragma unroll
         for (int k = 0; k < V; ++k) v[k] *= f;
-        store_vec<T, V>(dst + (size_t)i * V, v);
+        if (NT) store_vec_nt<T, V>(dst + (size_t)i * V, v);
+        else store_vec<T, V>(dst + (size_t)i * V, v);
     }
     const uint32_t t = nv * V + threadIdx.x;
     if (t < n) dst[t] = (T)((float)src[t] * f);
 }
 
-template <typename TABLE_T>
+template <bool NT, typename TABLE_T>
 __global__ void __launch_bounds__(256) grad_scale_kernel(const TABLE_T t, const ClipArgs a) {
     __shared__ double lds4[4];
     const Chunk c = chunk_of(t, blockIdx.x);
     const float f = clip_factor(a, lds4) * a.s0;
     if (f == 1.f && c.src == c.dst) return;   // in place and nothing to do
-    if (c.type == SR_T_F32) scale_run((const float*)c.src, (float*)c.dst, c.n, f);
-    else if (c.type == SR_T_BF16) scale_run((const bf16_t*)c.src, (bf16_t*)c.dst, c.n, f);
-    else scale_run((const f16_t*)c.src, (f16_t*)c.dst, c.n, f);
+    if (c.type == SR_T_F32) scale_run<NT>((const float*)c.src, (float*)c.dst, c.n, f);
+    else if (c.type == SR_T_BF16) scale_run<NT>((const bf16_t*)c.src, (bf16_t*)c.dst, c.n, f);
+    else scale_run<NT>((const f16_t*)c.src, (f16_t*)c.dst, c.n, f);
 }
 
 // an empty list has no chunks, but still a norm
@@ -219,6 +226,7 @@ struct sr_tensors {
     std::vector<uint32_t> first;             // first partial sum of every tensor, and their number
     std::vector<std::pair<const char*, const char*>> sorted;   // byte ranges by address
     uint32_t chunk = 0;
+    int64_t bytes = 0;
     bool overlap = false;                    // two tensors share memory
     Record* d_records = nullptr;             // of every chunk (sr_tensors_upload), behind them `first`
 };
@@ -268,7 +276,8 @@ hipError_t launch_list(const sr_tensors* t, const sr_tensors* out, void* ws, con
     if (!blocks) return hipSuccess;
     auto run = [&](const auto& table) {
         grad_partials_kernel<<<blocks, 256, 0, st>>>(table, (double*)ws);
-        if (c) grad_scale_kernel<<<blocks, 256, 0, st>>>(table, *c);
+        if (c && t->bytes > PAST_CACHES) grad_scale_kernel<true><<<blocks, 256, 0, st>>>(table, *c);
+        else if (c) grad_scale_kernel<false><<<blocks, 256, 0, st>>>(table, *c);
         return hipGetLastError();
     };
     bool have;
@@ -351,6 +360,7 @@ int sr_tensors_create(sr_tensors** out, int device, int n, const sr_tensor_desc*
                 parts += (uint32_t)grad_chunks(m, t->chunk);
             }
             t->first.push_back(parts);
+            t->bytes += d.count * b;
             if (d.count) t->sorted.emplace_back((const char*)d.data, (const char*)d.data + d.count * b);
         }
         std::sort(t->sorted.begin(), t->sorted.end());

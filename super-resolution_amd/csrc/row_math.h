@@ -31,6 +31,19 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[N]) {
     *reinterpret_cast<Vec<T, N>*>(p) = x;
 }
 
+// ... a 16-byte store that passes the caches by
+template <typename T, int N>
+__device__ __forceinline__ void store_vec_nt(T* p, const float (&v)[N]) {
+    static_assert(N * sizeof(T) == 16, "one vector");
+    typedef unsigned U4 __attribute__((ext_vector_type(4), aligned(2)));
+    Vec<T, N> x;
+#pragma unroll
+    for (int k = 0; k < N; ++k) x.v[k] = (T)v[k];
+    U4 b;
+    __builtin_memcpy(&b, &x, 16);
+    __builtin_nontemporal_store(b, reinterpret_cast<U4*>(p));
+}
+
 template <int CTRL>
 __device__ __forceinline__ float dpp_add(float v) {
     return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xF, 0xF, true));
