@@ -43,7 +43,7 @@ class TecoGAN(FrameRecurrentVideoSR):
         train_cfg = (self.configs.get('train') or {}) if isinstance(self.configs, dict) else {}
         self.tecogan = TecoGANModel(self.generator, self.discriminator,
                                     train_discriminator=train_cfg.get('gan_updates_discriminator', True))
-        self.opt = Adam(lr=5e-5, clipnorm=self._clipnorm())                                    # ONE instance for the three models, TecoGAN.py:110-131
+        self.opt = Adam(lr=5e-5, clipnorm=self._clipnorm())      # ONE instance for the three models, TecoGAN.py:110-131
         self.generator.compile(loss=['mean_squared_error', 'mean_squared_error'], loss_weights=[1., 1.], optimizer=self.opt)
         self.discriminator.compile(loss=['binary_crossentropy'] + ['mean_squared_error'] * 4,
                                    loss_weights=[1., 0., 0., 0., 0.], optimizer=self.opt)

@@ -30,6 +30,7 @@ struct sr_train_state {
     int64_t t = 0;                      // optimizer iterations
     float *d_m2 = nullptr, *d_v2 = nullptr;   // Adam moments of the generator inside tecogan.train_on_batch (its own train function)
     double* clip_parts = nullptr;       // partial sums of a clipped step (two vectors), the norm behind them; allocated by the first one
+    hipEvent_t ev_clip = nullptr;       // the discriminator's step of a combined one has read the partial sums
     bool clipped = false;               // there was one
     bool host_stale = false;            // ctx->tensors older than d_params
     ConvLayer fnet_dg[14], srnet_dg[24];   // data-gradient convs of the Conv2D layers (planned where needed)
@@ -702,7 +703,8 @@ void train_free(sr_ctx* c) {
         }
     if (T->h_stage) (void)hipHostFree(T->h_stage);
     if (T->h_loss) (void)hipHostFree(T->h_loss);
-    if (T->ev_start) (void)hipEventDestroy(T->ev_start);
+    for (hipEvent_t e : {T->ev_start, T->ev_clip})
+        if (e) (void)hipEventDestroy(e);
     for (int k = 0; k < sr_train_state::MAX_UP; ++k)
         for (hipEvent_t e : {T->ev_est[k], T->ev_hr[k]})
             if (e) (void)hipEventDestroy(e);
@@ -1275,8 +1277,13 @@ static int tecogan_adam(sr_ctx* c, sr_disc* d, const float* d_gen_grads, const f
     if (train_disc) {
         HIPCHK(c, hipStreamSynchronize(c->stream));
         HIPCHK(c, hipStreamSynchronize(d->stream));
-        if ((rc = disc_apply(d, d_disc_grads, scale_d, lr, beta1, beta2, eps, t, 1, false, true, clipping ? &clip : nullptr)))
-            return fail(c, rc, "%s", d->err.c_str());
+        rc = disc_apply(d, d_disc_grads, scale_d, lr, beta1, beta2, eps, t, 1, false, true, clipping ? &clip : nullptr);
+        if (clipping && d->stream != c->stream) {     // the next clipped step of this ctx writes the partial sums that this one reads
+            if (!T->ev_clip) HIPCHK(c, hipEventCreateWithFlags(&T->ev_clip, hipEventDisableTiming));
+            HIPCHK(c, hipEventRecord(T->ev_clip, d->stream));
+            HIPCHK(c, hipStreamWaitEvent(c->stream, T->ev_clip, 0));
+        }
+        if (rc) return fail(c, rc, "%s", d->err.c_str());
     }
     return SR_OK;
 }

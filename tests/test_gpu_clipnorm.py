@@ -160,6 +160,43 @@ def test_combined_step_clips_both_models_by_one_norm(sh, weights7, train_disc):
         q.close()
 
 
+def test_generator_step_right_behind_a_combined_one(sh, weights7):
+    """The discriminator's part of a combined step runs on its own stream and reads the ctx's partial sums; the ctx's next step, which
+    writes them anew, comes behind it."""
+    import torch
+    B, h, w = 1, 16, 16
+    rng = np.random.default_rng(4)
+    pairs = []
+    for _ in range(2):
+        ctx, d = context(sh, weights7, "tecogan", h, w), sh.Discriminator(4 * h, 4 * w, max_batch=B)
+        d.load_weights(rd.make_disc_weights(6, 4 * h, 4 * w))
+        pairs.append((ctx, d))
+    (ctx, d), (ctx2, d2) = pairs
+    lr = [rng.random((B, h, w, 3), dtype=np.float32) for _ in range(2)]
+    hr = [rng.random((B, 4 * h, 4 * w, 3), dtype=np.float32) for _ in range(7)]
+    feats = [rng.standard_normal((B, 64 >> (k + 1), 64 >> (k + 1), c)).astype(np.float32) for k, c in enumerate((64, 64, 128, 256))]
+    for c, q in pairs:
+        sh.tecogan_grads(c, q, lr[0], lr[1], *hr, feats, hr[6][::-1].copy(), rd.LOSS_WEIGHTS)
+        c.set_clipnorm(1e-2)
+    g, gd = (torch.from_numpy(f).cuda() for f in (ctx.train_read_grads(), d.read_grads()))
+    other = 50 * g                              # another norm for the generator's own steps
+    torch.cuda.synchronize()
+    for t in range(1, 9):
+        for c, q in pairs:
+            sh.tecogan_apply(c, q, t, d_gen_grads=g.data_ptr(), d_disc_grads=gd.data_ptr())
+            if c is ctx2:
+                torch.cuda.synchronize()
+            c.train_apply(d_grads=other.data_ptr())
+            if c is ctx2:
+                torch.cuda.synchronize()
+    assert ctx.grad_norm() == ctx2.grad_norm() > 1e-2
+    same_weights(ctx, ctx2)
+    same_weights(d, d2)
+    for c, q in pairs:
+        c.close()
+        q.close()
+
+
 def test_refusals(sh, weights7):
     c = context(sh, weights7)
     d = sh.Discriminator(16, 16)
