@@ -6,8 +6,8 @@
 // there) and writes it once.  The squares are added in 64 bits: an fp32 square overflows above 1.8e19 and vanishes below 1e-23, a
 // 64-bit one does neither, and beside the loads the conversions and products cost nothing (250 M bf16 elements: 84 us, 5.9 TB/s).
 // A tensor is cut into chunks, a workgroup takes one chunk and leaves one partial sum; chunks grow with the whole list so that there
-// are about 4096 of them at most, which every workgroup of the clipping launch adds up by itself in one fixed order (32 KB from L2)
-// -- no atomics, no third launch, the same bits on every run.
+// are about 4096 of them at most (and one a tensor), added up in one fixed order: no atomics, the same bits on every run.  Every
+// workgroup of the clipping launch does that by itself where they are few, which saves a launch.
 #include "grad_clip.h"
 #include "op_host.h"
 #include "row_math.h"
@@ -32,6 +32,10 @@ constexpr int TABLE = 160;
 // types: 106 -> 84 us, 100 M bf16: 128 -> 106; 250 M bf16 at odd addresses: 315 -> 322; 5 M fp32 would gain 1 us and lose it to the
 // next reader).
 constexpr int64_t PAST_CACHES = 128 << 20;
+// From this many partial sums on, a launch of one workgroup joins them before the clipping one (2 us): each of that one's workgroups
+// would read them all, which grows with the square (us without / with, to other tensors: 24 M fp32 in 2929 sums 46.6 / 48.4, 33 M in
+// 4028 sums 64.7 / 63.6, 33 M bf16 39.2 / 36.4, 10,000 tensors of 1000 fp32 64 / 31, 60,000 of 100 1541 / 118).
+constexpr uint32_t JOIN_FROM = 3600;
 
 struct Piece {
     const void* src;
@@ -175,6 +179,20 @@ __global__ void __launch_bounds__(256) grad_scale_kernel(const TABLE_T t, const 
     else scale_run<NT>((const f16_t*)c.src, (f16_t*)c.dst, c.n, f);
 }
 
+// all partial sums to one behind them
+__global__ void __launch_bounds__(1024) grad_join_kernel(double* __restrict__ parts, uint32_t n) {
+    __shared__ double lds[16];
+    double s = 0.0;
+#pragma unroll 8
+    for (uint32_t i = threadIdx.x; i < n; i += 1024) s += parts[i];
+    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int w = 1; w < 16; ++w) s += lds[w];
+    parts[n] = s;
+}
+
 // an empty list has no chunks, but still a norm
 __global__ void grad_zero_norm_kernel(float* norm) { *norm = 0.f; }
 
@@ -245,7 +263,7 @@ std::mutex g_retired_mu;
 std::vector<std::pair<int, Record*>> g_retired;
 
 // workspace: the partial sums; for a list that does not fit the kernel arguments, the records of both sides
-size_t parts_bytes(const sr_tensors* t) { return std::max<size_t>(t->first.back(), 1) * sizeof(double); }
+size_t parts_bytes(const sr_tensors* t) { return ((size_t)t->first.back() + 1) * sizeof(double); }
 size_t workspace_of(const sr_tensors* t) {
     return parts_bytes(t) + (t->pieces.size() > TABLE ? 2 * t->first.back() * sizeof(Record) : 0);
 }
@@ -275,9 +293,16 @@ hipError_t launch_list(const sr_tensors* t, const sr_tensors* out, void* ws, con
     const uint32_t blocks = t->first.back();
     if (!blocks) return hipSuccess;
     auto run = [&](const auto& table) {
-        grad_partials_kernel<<<blocks, 256, 0, st>>>(table, (double*)ws);
-        if (c && t->bytes > PAST_CACHES) grad_scale_kernel<true><<<blocks, 256, 0, st>>>(table, *c);
-        else if (c) grad_scale_kernel<false><<<blocks, 256, 0, st>>>(table, *c);
+        double* parts = (double*)ws;
+        grad_partials_kernel<<<blocks, 256, 0, st>>>(table, parts);
+        if (!c) return hipGetLastError();
+        ClipArgs a = *c;
+        if (blocks > JOIN_FROM) {
+            grad_join_kernel<<<1, 1024, 0, st>>>(parts, blocks);
+            a.parts = parts + blocks, a.n0 = 1;
+        }
+        if (t->bytes > PAST_CACHES) grad_scale_kernel<true><<<blocks, 256, 0, st>>>(table, a);
+        else grad_scale_kernel<false><<<blocks, 256, 0, st>>>(table, a);
         return hipGetLastError();
     };
     bool have;

@@ -105,6 +105,42 @@ def test_views_into_a_buffer_leave_the_rest(sh):
                 assert bool((dst == -3.0).all())
 
 
+@pytest.mark.parametrize("dt", [F32, F16])
+@pytest.mark.parametrize("upload", [True, False])
+def test_thousands_of_tensors(sh, dt, upload):
+    """A partial sum a tensor: these are joined before the clipping launch."""
+    sizes = [1 + i * 7 % 900 for i in range(9000)]
+    flat = randn(2, sum(sizes), scale=0.1).to(dt)
+    ts, dst = list(torch.split(flat, sizes)), torch.full_like(flat, 9.0)
+    lst, out = sh.TensorList(ts, upload=upload), sh.TensorList(list(torch.split(dst, sizes)), upload=upload)
+    want = norm64([flat])
+    for share in (0.3, 3.0):
+        norm = sh.clip_grads(lst, share * want, out=out)
+        check_norm(norm, want)
+        check_clipped(dst, flat, want, share * want, 1.0)
+    keep = flat.clone()
+    check_norm(sh.clip_grads(lst, want / 8, scale=0.5), want / 2)
+    check_clipped(flat, keep, want / 2, want / 8, 0.5)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_large_lists_stored_past_the_caches(sh, dt):
+    """More than 128 MB: in place, and into views at odd addresses, whose surroundings stay."""
+    sizes = [1, 30_000_001, 4099, 45_000_007]
+    ts = [randn(i, n, scale=0.1).to(dt) for i, n in enumerate(sizes)]
+    whole = torch.full((sum(sizes) + 3,), -3.0, dtype=dt, device="cuda")
+    out = list(torch.split(whole[1:-2], sizes))
+    want = norm64(ts)
+    norm = sh.clip_grads(sh.TensorList(ts), want / 3, out=sh.TensorList(out))
+    check_norm(norm, want)
+    for o, t in zip(out, ts):
+        check_clipped(o, t, want, want / 3, 1.0)
+    assert float(whole[0]) == -3.0 and bool((whole[-2:] == -3.0).all())
+    assert torch.equal(sh.clip_grads(ts, want / 3), norm)
+    for o, t in zip(out, ts):
+        assert torch.equal(o, t)
+
+
 def test_any_dense_order_of_dimensions(sh):
     t = randn(3, 5, 4, 6, 7)
     p = t.permute(0, 3, 1, 2)
