@@ -406,7 +406,7 @@ int sr_op_conv3x3_wgrad_noalloc(int device, int dtype, int B, int H, int W, int 
 
 /* ---- operators of a residual trunk and of its training step on DEVICE tensors (no counterpart in the reference) --------------
  * What a deeper trunk of residual blocks (reference layers.py:58-62) needs to stay trainable: norms before and after a block, and
- * gradients clipped by their global norm.  All calls take DEVICE pointers, are asynchronous on `hip_stream` (a hipStream_t of
+ * gradients clipped by their global norm.  The sr_op_* calls take DEVICE pointers, are asynchronous on `hip_stream` (a hipStream_t of
  * `device`, NULL = its default stream), allocate nothing, keep nothing and can be captured into a HIP graph.  `device` need not be
  * the caller's current device, which is restored on every path.  A workspace belongs to one call at a time: two calls that may
  * overlap (on two streams, in two graphs) need one each.  Results do not depend on the run: no atomics, sums in a fixed order. */
@@ -423,8 +423,8 @@ enum sr_gate_act { SR_GATE_LINEAR = 0, SR_GATE_SIGMOID = 1 };
  * `rows_per_gate` consecutive rows share a gate row (1: a gate value for every element; h * w: a channel gate for every image); it
  * divides `rows` and is not looked at without a gate.  x, h, dx, dh have the stream's type; y, gate, n and their gradients the
  * branch's, which is the stream's or, beside an fp32 stream, a 16-bit one; gains, biases and their gradients are dense fp32
- * vectors, NULL = ones / zeros.  ld*: elements between rows (>= channels; the channels of a row are contiguous, any alignment of
- * whole elements).  Sums and all values in between are fp32, with squares up to 3e38: |v| beyond 1e18 overflows them.
+ * vectors, NULL = ones / zeros.  ld*: elements between rows (channels .. 2^31 - 1; the channels of a row are contiguous, any alignment
+ * of whole elements).  Sums and all values in between are fp32, with squares up to 3e38: |v| beyond 1e18 overflows them.
  * sr_op_residual_norm: without a branch (y NULL: norms == SR_NORM_PRE, no gate) h is x and is not written.  h may be x or y, n may
  *   be x or y (same type and pitch), gate too with rows_per_gate 1; otherwise outputs overlap nothing.
  * sr_op_residual_norm_bwd: from h (needed with SR_NORM_PRE), y (with SR_NORM_POST or a gate), dh = the gradient that reaches h

@@ -909,8 +909,15 @@ _torch = None
 _torch_types = None
 _current_stream = None
 _bwd_bytes = {}      # bytes of workspace of the backward calls made so far
-# sr_residual_norm_desc: rows, rows_per_gate, ten pitches; channels, stream_type, branch_type, kind, norms, gate_act; scale, eps
-_pack_block = struct.Struct("=12q6i2f").pack
+_block_desc = struct.Struct("=12q6i2f")      # sr_residual_norm_desc
+
+
+def _pack_block(*fields):
+    """rows, rows_per_gate, ten pitches; channels, stream_type, branch_type, kind, norms, gate_act; scale, eps"""
+    try:
+        return _block_desc.pack(*fields)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"scale and eps must be finite float32 numbers: {e}") from None
 
 
 class _TensorDesc(C.Structure):
@@ -999,7 +1006,14 @@ def _gate_rows(gate, shape, rows, dtype, dev):
     C_ = shape[-1]
     if gate.dim() == 0 or gate.shape[-1] != C_:
         raise ValueError(f"gate: expected {C_} channels in the last dimension, got shape {tuple(gate.shape)}")
-    gates = gate.numel() // C_
+    gates, gs = gate.numel() // C_, gate.shape
+    if gate.dim() > 2 and gs != shape:
+        # (B, 1, 1, C): a row for every leading index of the stream, shared by consecutive rows; other dimensions cannot share one
+        lead = 0
+        while lead < min(len(gs), len(shape)) - 1 and gs[lead] == shape[lead]:
+            lead += 1
+        if len(gs) != len(shape) or any(n != 1 for n in gs[lead:-1]):
+            raise ValueError(f"gate: expected (G, {C_}), {tuple(shape)} or its leading dimensions with ones behind them, got {tuple(gs)}")
     if (rows % gates if gates else rows) != 0:
         raise ValueError(f"gate: {gates} rows do not divide the {rows} rows of the stream")
     return rows // gates if rows else 1, _pitch(gate, "gate", gate.shape, dtype, dev)
@@ -1009,10 +1023,11 @@ def residual_norm(x, y=None, gate=None, post_gain=None, post_bias=None, pre_gain
                   gate_act="linear", scale=1.0, eps=1e-6, branch_dtype=None, h=None, n=None, stream=None):
     """A residual block's output joined to its stream, with the norm behind the block and the one before the next
     (include/sr_hip.h sr_op_residual_norm): h = x + scale * act(gate) * post(y), n = pre(h).  Torch tensors on one GPU, x (..., C)
-    the stream, y of the same shape the block's output; gate of the same shape, or (G, C) where G divides the rows: (B, C) gates
-    the channels of each image of an NHWC batch.  norms 'both', 'post' or 'pre', kind 'rms' or 'layer', gains and biases float32.
-    Without y: n = pre(x) in branch_dtype (default x's), and h is x.  h, n: tensors to write (h may be x, n may be y), default new
-    ones.  Returns (h, n), n None with norms 'post'.  Runs on `stream` (a hipStream_t as int), default torch's current one."""
+    the stream, y of the same shape the block's output; gate of the same shape, or (G, C) where G divides the rows and rows / G of
+    them in a row share one: (B, C), or (B, 1, 1, C), gates the channels of each image of an NHWC batch.  norms 'both', 'post' or
+    'pre', kind 'rms' or 'layer', gains and biases float32.  Without y: n = pre(x) in branch_dtype (default x's), and h is x.  h, n:
+    tensors to write (h may be x, n may be y), default new ones.  Returns (h, n), n None with norms 'post'.  Runs on `stream` (a
+    hipStream_t as int), default torch's current one."""
     if stream is not None:
         with _on(stream, x.device):
             return residual_norm(x, y, gate, post_gain, post_bias, pre_gain, pre_bias, norms, kind, gate_act, scale, eps, branch_dtype, h, n)
@@ -1131,8 +1146,9 @@ def residual_norm_bwd(h, y=None, dh=None, dn=None, gate=None, post_gain=None, po
 class TensorList:
     """Dense torch tensors on one GPU -- a model's gradients -- as grad_norm and clip_grads take them (include/sr_hip.h
     sr_tensors_create).  Any mix of float32, bfloat16 and float16, any sizes (0 too), any order of dimensions as long as the
-    elements leave no gaps.  Holds on to the tensors; a program whose gradients stay in the same buffers makes it once.  upload: leave
-    what the kernels need to know of the list on the GPU (sr_tensors_upload), not while a stream is captured."""
+    elements leave no gaps.  Holds on to the tensors and the memory that they have now; a program whose gradients stay in the same
+    buffers makes it once.  upload: leave what the kernels need to know of the list on the GPU (sr_tensors_upload), not while a
+    stream is captured."""
 
     def __init__(self, tensors, upload=True):
         self.tensors = list(tensors)
@@ -1148,6 +1164,8 @@ class TensorList:
             if not _dense(t):
                 raise ValueError(f"tensor {i} of shape {tuple(t.shape)} and strides {tuple(t.stride())} has gaps or repeats elements")
             desc[i].data, desc[i].count, desc[i].type = t.data_ptr() or None, t.numel(), _type_of(t.dtype, f"tensor {i}")
+        # a tensor that is given other memory (t.data = ...) leaves this behind
+        self._storages = [t.untyped_storage() for t in self.tensors] if upload else None
         self._h = _vp()
         _check(lib().sr_tensors_create(C.byref(self._h), self.device.index, len(self.tensors), desc))
         need = C.c_size_t()
@@ -1162,7 +1180,7 @@ class TensorList:
     def close(self):
         if getattr(self, "_h", None):
             lib().sr_tensors_destroy(self._h)
-            self._h = None
+            self._h = self._storages = None
 
     def __del__(self):
         try:

@@ -195,9 +195,11 @@ def test_backward(sh, C, types):
         check_bwd(sh, c, norms, kind, ["linear", "sigmoid"][i % 2])
 
 
-@pytest.mark.parametrize("lead,C,gate", [((40, 640), 64, 40), ((7, 1000), 48, 7), ((1500, 3), 64, 1500), ((3000,), 520, 1), ((2, 1300), 1030, 2)])
+@pytest.mark.parametrize("lead,C,gate", [((40, 640), 64, 40), ((7, 1000), 48, 7), ((1500, 3), 64, 1500), ((3000,), 520, 1), ((2, 1300), 1030, 2), ((2100, 2), 521, 2100),
+                                         ((600, 2), 4100, 600), ((2, 4, 300), 250, 2)])
 def test_backward_many_rows(sh, lead, C, gate):
-    """Several workgroups to a gate row, several gate rows to a workgroup, gate rows that are whole in one."""
+    """Several workgroups to a gate row, several gate rows to a workgroup (which then adds to its partial sums), gate rows that are
+    whole in one."""
     check_bwd(sh, case(5, lead, C, F32, F32, gate), "both", "layer", "sigmoid")
     check_bwd(sh, case(6, lead, C, BF16, BF16, "element"), "both", "rms", "linear")
 
@@ -395,9 +397,18 @@ def test_refusals(sh):
     for bad in (dict(gate=torch.zeros(4, 16, device="cuda")), dict(gate=torch.zeros(6, 8, device="cuda")), dict(post_gain=torch.ones(8, device="cuda")),
                 dict(pre_gain=w.bfloat16()), dict(pre_bias=torch.zeros(16)), dict(eps=0.0), dict(eps=float("nan")), dict(scale=float("inf")),
                 dict(norms="none"), dict(kind="batch"), dict(gate_act="relu"), dict(h=y.t().contiguous().t()), dict(h=torch.zeros(6, 16, device="cuda", dtype=BF16)),
-                dict(h=y[:3]), dict(n=x[:, ::2])):
+                dict(h=y[:3]), dict(n=x[:, ::2]), dict(scale=1e300), dict(gate=torch.zeros(2, 1, 16, device="cuda"))):
         with pytest.raises(ValueError):
             sh.residual_norm(x, y, **{**ok, **bad})
+    x4 = torch.zeros(2, 3, 3, 16, device="cuda")
+    for g in ((2, 16), (2, 1, 1, 16), (2, 3, 1, 16), (2, 3, 3, 16), (1, 16), (6, 16), (1, 1, 1, 16)):
+        sh.residual_norm(x4, x4, gate=torch.zeros(*g, device="cuda"), **ok)
+    for g in ((3, 16), (4, 16), (1, 3, 3, 16), (2, 1, 3, 16), (3, 3, 16), (1, 1, 16), (2, 3, 16), (9, 1, 1, 16)):
+        if g == (3, 16):
+            sh.residual_norm(x4, x4, gate=torch.zeros(*g, device="cuda"), **ok)      # (G, C): any number of rows that divides 18
+            continue
+        with pytest.raises(ValueError, match="gate"):
+            sh.residual_norm(x4, x4, gate=torch.zeros(*g, device="cuda"), **ok)
     flat = torch.zeros(400, device="cuda")
     with pytest.raises(ValueError, match="overlaps"):      # one element further on
         sh.residual_norm(flat[:96].view(6, 16), y, h=flat[1:97].view(6, 16), **ok)
