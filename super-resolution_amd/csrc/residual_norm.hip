@@ -15,8 +15,8 @@
 // once: a group of lanes (a "team") holds it in registers across all sums of the row, and the backward pass takes the row
 // statistics again from what it holds instead of reading them.  Rows of up to 512 channels belong to 1..64 lanes of a wave, several
 // rows to a wave, and their sums are lane exchanges; longer rows belong to a workgroup, which joins its waves' sums in LDS.  A lane
-// holds 8 elements of a row (4 in the backward pass of long rows, which otherwise spills: 8192 x 1000 takes 43 us instead of 50) and has
-// the same places of the team's next row on their way.  All sums and the values between them are fp32; tensors of 16 bits are rounded
+// holds 8 elements of a row (4 in the backward pass of long rows where 8 need more registers than there are) and has the same places of
+// the team's next row on their way.  All sums and the values between them are fp32; tensors of 16 bits are rounded
 // once, when they are stored.
 #include "op_host.h"
 #include "row_math.h"
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(BLK ? 1024 : 256) rn_fwd_kernel(const FwdArgs 
 }
 
 // ------------------------------------------------------------------------------------------------- backward
-// The sums over rows that a thread keeps for its 8 columns, in LDS: in registers the four of them would cost a wave in four, and
+// The sums over rows that a thread keeps for its columns, in LDS: in registers the four of them would cost a wave in four, and
 // LDS has the time (two 16-byte reads and writes a sum and row, under a tenth of what the row takes to arrive).
 // [sum][half][thread] float4: no bank conflicts, and each thread's are its own until they are joined.
 template <int E>
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(BLK ? 1024 : 256, BLK ? 4 : 3) rn_bwd_kernel(c
             sums.get(S_PW, v);
             sums.get(S_PB, w);
             load_gain(a.pb, t, pb, 0.f);
-            // a slot that no other sum needs takes dgate: S_PB where the bias has no gradient, else behind the rest
+            // S_PB's place takes dgate until it is out
 #pragma unroll
             for (int k = 0; k < E; ++k) {
                 pb[k] = (a.flags & F_POST ? pw[k] * v[k] + pb[k] * w[k] : v[k]) * (a.flags & F_SIGMOID ? act[k] * (1.f - act[k]) : 1.f);
@@ -595,8 +595,8 @@ __global__ void __launch_bounds__(BLK ? 1024 : 256, BLK ? 4 : 3) rn_bwd_kernel(c
 
 // The partial sums of a backward pass joined in a fixed order: 4 columns a thread, LC threads side by side, 1024 / LC slices of the
 // partial sums.  16 threads side by side read 256 bytes at a time (24 MB of sums for 6000 channels: 7.0 us, with 4 threads 12.9), 4
-// give four times the workgroups where the columns are few (2 x 771: 5.4 us instead of 12.4).  blockIdx.y < 4: the gradient of that gain or bias over the workgroups; beyond: gate row blockIdx.y - 4 over its
-// units.
+// give four times the workgroups where the columns are few (2 x 771: 5.4 us instead of 12.4).  blockIdx.y < 4: the gradient of that
+// gain or bias over the workgroups; beyond: gate row blockIdx.y - 4 over its units.
 struct JoinArgs {
     const float* part;
     float* out[4];
@@ -682,15 +682,17 @@ struct Split {
     bool shared_gate = false;
 };
 
-// `waves`: how many waves of the kernel a CU holds at once.  The workgroups are as many as that gives: a few more would cost a
-// second round of them, and with many more a team has too few rows to have the next one on its way (16384 x 4096 bf16 forward: 100
-// us with 16 waves a CU, 105 with 48, 112 with one row a workgroup)
-Split split_of(const sr_residual_norm_desc* d, const Shape& s, bool gate, unsigned rpg, int waves) {
+// `waves`: how many waves of the kernel a CU holds at once; `tight`: a quarter of them on each of its four SIMDs and no more, so that a workgroup of 5 waves,
+// which is two waves to one of them, fits twice and not three times (11648 x 1030 bf16 gated backward: 87 -> 70 us).  The workgroups are
+// as many as that gives: a few more would cost a second round of them, and with many more a team has too few rows to have the next
+// one on its way (16384 x 4096 bf16 forward: 100 us with 16 waves a CU, 105 with 48, 112 with one row a workgroup)
+Split split_of(const sr_residual_norm_desc* d, const Shape& s, bool gate, unsigned rpg, int waves, bool tight) {
     Split p;
     if (d->rows == 0) return p;
     p.shared_gate = gate && rpg > 1;
     p.u.span = p.shared_gate ? rpg : (unsigned)d->rows;
-    const int64_t groups = d->rows / p.u.span, resident = 256 * std::max(1, waves * 64 / s.threads);
+    const int wg = s.threads / 64, fit = tight && wg > 4 ? waves / 4 / ((wg + 3) / 4) : waves / wg;
+    const int64_t groups = d->rows / p.u.span, resident = 256 * std::max(1, fit);
     const int64_t most = (p.u.span + s.teams - 1) / s.teams;
     p.u.per_group = (unsigned)std::min(most, std::max<int64_t>(1, resident / groups));
     p.u.units = (unsigned)(groups * p.u.per_group);
@@ -734,8 +736,10 @@ void launch_bwd(const BwdArgs& a, int blocks, int threads, hipStream_t st) {
 
 template <typename TS, typename TB, int E, int VEC, bool BLK, bool TAIL>
 void launch_bwd(const BwdArgs& a, int gate, bool full, int blocks, int threads, hipStream_t st) {
-    if (gate == G_NONE) full ? launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_NONE, true>(a, blocks, threads, st) : launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_NONE, false>(a, blocks, threads, st);
-    else if (gate == G_ROW) full ? launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_ROW, true>(a, blocks, threads, st) : launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_ROW, false>(a, blocks, threads, st);
+    if (gate == G_NONE) {
+        if constexpr (E == 8 || sizeof(TS) == 4)      // see bwd_plan
+            full ? launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_NONE, true>(a, blocks, threads, st) : launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_NONE, false>(a, blocks, threads, st);
+    } else if (gate == G_ROW) full ? launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_ROW, true>(a, blocks, threads, st) : launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_ROW, false>(a, blocks, threads, st);
     else full ? launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_SHARED, true>(a, blocks, threads, st) : launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_SHARED, false>(a, blocks, threads, st);
 }
 
@@ -756,9 +760,18 @@ struct BwdPlan {
 
 BwdPlan bwd_plan(const sr_residual_norm_desc* d, bool gate, unsigned rpg, bool full) {
     BwdPlan q;
-    const bool simple = !full && !gate && d->channels % 8 == 0;
-    q.s = shape_of(d, d->channels <= WAVE_C || d->channels > 4096 || simple ? 8 : 4);
-    q.p = split_of(d, q.s, gate, rpg, q.s.blk || simple ? 16 : 12);
+    const int C = d->channels;
+    const bool whole8 = C % 8 == 0, whole4 = C % 4 == 0;
+    // 8 elements a lane are fewer waves to a row and so more rows at a time, but with a gate or fp32 tensors more than the registers
+    // hold.  us at 12 M elements, 8 elements a lane / 4:
+    //   16 bits, no gate:      776 channels rms 35.5 / 37.5, layer 43 / 49; 1541: 37 / 46, 49 / 60; 4095: 39 / 45, 54 / 58
+    //   16 bits, gated, % 8:   640: 54.6 / 51.0; 1304: 51 / 59; 2312: 50 / 61; 3400: 49 / 53;   other channels: 1541: 64 / 59; 4095: 68 / 57
+    //   fp32, no gate, % 4, where 4 elements make rows of 9 to 12 waves, of which a CU holds one: 2056: 53 / 68, layer 63 / 75; 2600:
+    //   55 / 62, 66 / 69;   else: 776: 59.9 / 56.3, 76 / 60; 1544: 57.6 / 53.7; 3400: 57 / 59, 69 / 67;   other channels: 2050: 66 / 54
+    const int wide = (C + 255) / 256;
+    const bool e8 = d->stream_type == SR_T_F32 ? !gate && whole4 && wide > 8 && wide <= 12 : !gate || (whole8 && C > 1024);
+    q.s = shape_of(d, C <= WAVE_C || C > 4096 || e8 ? 8 : 4);
+    q.p = split_of(d, q.s, gate, rpg, q.s.blk || (!full && !gate && whole8) ? 16 : 12, q.s.e == 8 || !whole4);
     const size_t row = (size_t)round_up(d->channels, 4) * 4;
     q.part = round_up_sz((size_t)q.p.blocks * 4 * row);
     q.bytes = q.part + (q.p.shared_gate && q.p.u.per_group > 1 ? (size_t)q.p.u.units * row : 0);
@@ -845,7 +858,7 @@ extern "C" int sr_op_residual_norm(int device, const sr_residual_norm_desc* d, c
     RN_TRY(on.enter(device));
     if (d->rows == 0) return SR_OK;
     const Shape s = shape_of(d, 8);
-    const Split p = split_of(d, s, false, 1, 16);
+    const Split p = split_of(d, s, false, 1, 16, false);
     const int flags = (y ? F_BRANCH : 0) | (post ? F_POST : 0) | (pre ? F_PRE : 0) | (d->kind == SR_NORM_LAYER ? F_LAYER : 0) |
                       (d->gate_act == SR_GATE_SIGMOID ? F_SIGMOID : 0);
     const FwdArgs a = {x, y, gate, post ? post_gain : nullptr, post ? post_bias : nullptr, pre ? pre_gain : nullptr, pre ? pre_bias : nullptr,
