@@ -283,7 +283,7 @@ __device__ __forceinline__ void normalise(float (&v)[TEAM::E], const FwdArgs& a,
 }
 
 // The teams of all workgroups take the rows in turn, so that what is read at one time lies together: with a stretch of rows for each
-// workgroup instead, the 942,080 x 64 call took 195 us instead of 139.
+// workgroup instead, the 942,080 x 64 call with an fp32 stream took 195 us instead of 138 (5.2 TB/s; 16384 x 4096 bf16: 98 us, 5.5 TB/s).
 template <typename TS, typename TB, int E, int VEC, bool BLK, bool TAIL, int GATE>
 __global__ void __launch_bounds__(BLK ? 1024 : 256) rn_fwd_kernel(const FwdArgs a) {
     using TEAM = Team<E, VEC, BLK, TAIL>;
@@ -422,6 +422,7 @@ __device__ __forceinline__ void leave(int i, const Sums<TEAM::E>& sums, const TE
     }
 }
 
+// Rows in turn like the forward pass (8192 x 4096 bf16: 80.5 us, 5.0 TB/s; 163,840 x 64 fp32 with a gate an image: 50 us, 5.0 TB/s).
 // FULL: layer norms or gradients of biases; without, only what rms norms with gains need is in registers.  The sums over rows are
 // those of a unit; a workgroup with several units adds them up in its partial sums.  With a gate that a unit shares they are
 //   A = sum T hat(y) (or T y), B = sum T   (T with the scale):  dpost_gain = a A, dpost_bias = a B, dgate = a' (post_gain A + post_bias B)
