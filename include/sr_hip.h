@@ -431,7 +431,8 @@ enum sr_gate_act { SR_GATE_LINEAR = 0, SR_GATE_SIGMOID = 1 };
  *   through the stream (NULL: none; needed without SR_NORM_PRE) and dn (with SR_NORM_PRE) to dx = the whole gradient of h, dy (NULL:
  *   there is no branch), dgate (NULL: not wanted) and the vectors that are not NULL.  Row statistics are taken again from h and y.
  *   dx, dy may be h, y, dh or dn (same type and pitch).  rows == 0 zeroes the vectors.  `workspace`:
- *   sr_op_residual_norm_bwd_workspace bytes (gate: whether there is one), 16-byte aligned. */
+ *   sr_op_residual_norm_bwd_workspace bytes (gate: whether there is one; 0 where there are few rows: then it may be NULL),
+ *   16-byte aligned. */
 typedef struct sr_residual_norm_desc {
     int64_t rows, rows_per_gate;
     int64_t ldx, ldy, ldg, ldh, ldn;             /* x, y, gate, h, n */

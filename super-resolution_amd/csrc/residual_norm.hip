@@ -31,10 +31,12 @@ namespace {
 constexpr int MAX_C = 8192;          // 1024 lanes x 8 channels
 constexpr int WAVE_C = 512;          // up to here a row belongs to lanes of one wave
 
-enum Gate { G_NONE = 0, G_ROW = 1, G_SHARED = 2 };   // a gate row for every position / for several
+// no gate, a gate row for every position, for several, for a few (backward pass of rows within a wave)
+enum Gate { G_NONE = 0, G_ROW = 1, G_SHARED = 2, G_GROUP = 3 };
 
 // Work split of a backward pass: `per_group` workgroups share the `span` rows of a group (the rows that share a gate row, or all
-// rows); that is a unit each.  Their teams take the group's rows in turn, so that what is read at one time lies together.
+// rows); that is a unit each.  Their teams take the group's rows in turn, so that what is read at one time lies together.  With
+// G_GROUP a unit is a group, and the teams of all workgroups take the groups in turn.
 struct Units {
     unsigned span, units, per_group;
 };
@@ -56,13 +58,13 @@ struct BwdArgs {
     const void *h, *y, *gate, *dh, *dn;
     const float *pw, *pb, *qw;
     void *dx, *dy, *dgate;
-    float *part;                     // [blocks][nslot][pitch] partial sums of the gains' and biases' gradients
+    float *sums[4];                  // where the sums for post gain, post bias, pre gain, pre bias go (NULL: not wanted), `step` floats
+    int64_t step;                    // from workgroup to workgroup: partial sums, or the gradients themselves where there is one workgroup
     float *gpart;                    // [units][pitch] partial sums of dgate where a gate row spans several units
     int pitch;                       // C rounded up to 4: the sums are read 16 bytes at a time
     int ldh, ldy, ldg, lddh, lddn, lddx, lddy, lddg;
     Units u;
     int C, tl, flags;
-    int nslot, slot[4];              // where post gain, post bias, pre gain, pre bias are in `part`; -1: not wanted
     float scale, eps, inv_c;
 };
 
@@ -357,54 +359,71 @@ __global__ void __launch_bounds__(BLK ? 1024 : 256) rn_fwd_kernel(const FwdArgs 
 // ------------------------------------------------------------------------------------------------- backward
 // The sums over rows that a thread keeps for its columns, in LDS: in registers the four of them would cost a wave in four, and
 // LDS has the time (two 16-byte reads and writes a sum and row, under a tenth of what the row takes to arrive).
-// [sum][half][thread] float4: no bank conflicts, and each thread's are its own until they are joined.
-template <int E>
+// [wave][sum][half][lane] float4: no bank conflicts, and each thread's are its own until they are joined.  NS: how many sums
+template <int E, int NS>
 struct Sums {
-    static constexpr int Q = E / 4;
+    static constexpr int Q = E / 4, WAVE = NS * Q * 256;         // floats of a wave
     float4* at;
-    int step;
-    __device__ Sums(float* lds, int threads) : at(reinterpret_cast<float4*>(lds) + threadIdx.x), step(threads) {}
+    __device__ Sums(float* lds) : at(reinterpret_cast<float4*>(lds + (threadIdx.x >> 6) * WAVE) + (threadIdx.x & 63)) {}
+    // float k of quarter q of sum i of a lane of the first wave
+    static __device__ __forceinline__ int place(int i, int lane, int q, int k) { return ((Q * i + q) * 64 + lane) * 4 + k; }
     __device__ __forceinline__ void zero(int i) const {
 #pragma unroll
-        for (int q = 0; q < Q; ++q) at[(Q * i + q) * step] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int q = 0; q < Q; ++q) at[(Q * i + q) * 64] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     __device__ __forceinline__ void add(int i, const float (&v)[E]) const {
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
-            float4 a = at[(Q * i + q) * step];
+            float4 a = at[(Q * i + q) * 64];
             a.x += v[4 * q], a.y += v[4 * q + 1], a.z += v[4 * q + 2], a.w += v[4 * q + 3];
-            at[(Q * i + q) * step] = a;
+            at[(Q * i + q) * 64] = a;
         }
     }
     __device__ __forceinline__ void get(int i, float (&v)[E]) const {
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
-            const float4 a = at[(Q * i + q) * step];
+            const float4 a = at[(Q * i + q) * 64];
             v[4 * q] = a.x, v[4 * q + 1] = a.y, v[4 * q + 2] = a.z, v[4 * q + 3] = a.w;
         }
     }
     __device__ __forceinline__ void set(int i, const float (&v)[E]) const {
 #pragma unroll
-        for (int q = 0; q < Q; ++q) at[(Q * i + q) * step] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        for (int q = 0; q < Q; ++q) at[(Q * i + q) * 64] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
     }
 };
 
-// Column c of sum i over the teams of a workgroup of four waves
+// Few columns: 1 << splits() threads share one of `n`, each with a part of every wave's teams
 template <typename TEAM>
-__device__ __forceinline__ float joined(int i, int c, const TEAM& t, const float* lds) {
-    // element e of thread l of every team
-    const int l = c / TEAM::VEC % t.lanes, e = c / TEAM::VEC / t.lanes * TEAM::VEC + t.place(c);
-    const float* p = lds + ((Sums<TEAM::E>::Q * i + e / 4) * 256 + l) * 4 + e % 4;
-    float s = 0.f;
-#pragma unroll 8
-    for (int q = 0; q < t.rows; ++q) s += p[q * t.lanes * 4];
+__device__ __forceinline__ int splits(int n, const TEAM& t) {
+    int s = 0;
+    while (s < 6 - t.tl && n << (s + 1) <= (int)blockDim.x) ++s;
     return s;
+}
+
+// Column c of sum i over the teams of a workgroup, by 1 << s threads of which this is number k
+template <int NS, typename TEAM>
+__device__ __forceinline__ float joined(int i, int c, int k, int s, const TEAM& t, const float* lds) {
+    // element e of thread l of every team
+    const int j = c / TEAM::VEC, l = j & (t.lanes - 1), e = (j >> t.tl) * TEAM::VEC + t.place(c);
+    const float* p = lds + Sums<TEAM::E, NS>::place(i, l + k * t.lanes, e / 4, e % 4);
+    const int n = 64 >> (t.tl + s), step = t.lanes * 4 << s;
+    float v = 0.f;
+    for (int w = 0; w < (int)blockDim.x; w += 256, p += 4 * Sums<TEAM::E, NS>::WAVE) {     // four waves or eight
+#pragma unroll 2
+        for (int q = 0; q < n; ++q) {
+            float o[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) o[h] = p[q * step + h * Sums<TEAM::E, NS>::WAVE];
+            v += (o[0] + o[1]) + (o[2] + o[3]);
+        }
+    }
+    return s ? lanes_sum(v, s) : v;
 }
 
 // Sum i over the teams of a workgroup to out[0 .. C), on top of what is there with `add`; the same thread has the same column
 // every time
-template <typename T, typename TEAM>
-__device__ __forceinline__ void leave(int i, const Sums<TEAM::E>& sums, const TEAM& t, const float* lds, T* out, bool add) {
+template <int NS, typename T, typename TEAM>
+__device__ __forceinline__ void leave(int i, const Sums<TEAM::E, NS>& sums, const TEAM& t, const float* lds, T* out, bool add) {
     if constexpr (TEAM::BLK) {
         float v[TEAM::E], o[TEAM::E];
         sums.get(i, v);
@@ -415,9 +434,10 @@ __device__ __forceinline__ void leave(int i, const Sums<TEAM::E>& sums, const TE
         }
         store_row(out, t, v);
     } else {
-        for (int c = threadIdx.x; c < t.C; c += 256) {
-            const float s = joined(i, c, t, lds);
-            out[c] = (T)(add ? (float)out[c] + s : s);
+        const int s = splits(t.C, t), k = threadIdx.x & ((1 << s) - 1);
+        for (int c = threadIdx.x >> s; c < t.C; c += blockDim.x >> s) {
+            const float v = joined<NS>(i, c, k, s, t, lds);
+            if (k == 0) out[c] = (T)(add ? (float)out[c] + v : v);
         }
     }
 }
@@ -427,38 +447,43 @@ __device__ __forceinline__ void leave(int i, const Sums<TEAM::E>& sums, const TE
 // those of a unit; a workgroup with several units adds them up in its partial sums.  With a gate that a unit shares they are
 //   A = sum T hat(y) (or T y), B = sum T   (T with the scale):  dpost_gain = a A, dpost_bias = a B, dgate = a' (post_gain A + post_bias B)
 template <typename TS, typename TB, int E, int VEC, bool BLK, bool TAIL, int GATE, bool FULL>
-__global__ void __launch_bounds__(BLK ? 1024 : 256, BLK ? 4 : 3) rn_bwd_kernel(const BwdArgs a) {
+__global__ void __launch_bounds__(BLK ? 1024 : 512, BLK ? 4 : 3) rn_bwd_kernel(const BwdArgs a) {
     extern __shared__ float lds[];   // the sums, then BLK's [2][16][E] floats
-    enum { S_PW, S_QW, S_PB, S_QB };
+    constexpr bool ROW = GATE == G_ROW || GATE == G_GROUP;
+    constexpr int NS = (FULL ? 4 : GATE == G_SHARED ? 3 : 2) + (GATE == G_GROUP);
+    enum { S_PW, S_QW, S_PB, S_QB, S_GATE = NS - 1 };
     using TEAM = Team<E, VEC, BLK, TAIL>;
-    TEAM t(a.tl, a.C, lds + (FULL ? 4 : GATE == G_SHARED ? 3 : 2) * E * blockDim.x);
-    const Sums<E> sums(lds, BLK ? blockDim.x : 256);
+    TEAM t(a.tl, a.C, lds + NS * E * blockDim.x);
+    const Sums<E, NS> sums(lds);
     constexpr bool SUM_T = FULL || GATE == G_SHARED;
     float pw[E], qw[E];
     Raw<TS, TEAM> hr, dr;
     Raw<TB, TEAM> yr, nr, gr;
-    auto fetch = [&](unsigned r) {
+    auto fetch = [&](unsigned r, unsigned gate) {
         const TS *ph = row_of<const TS>(a.h, r, a.ldh), *pd = row_of<const TS>(a.dh, r, a.lddh);
-        const TB *py = row_of<const TB>(a.y, r, a.ldy), *pn = row_of<const TB>(a.dn, r, a.lddn), *pg = row_of<const TB>(a.gate, r, a.ldg);
+        const TB *py = row_of<const TB>(a.y, r, a.ldy), *pn = row_of<const TB>(a.dn, r, a.lddn), *pg = row_of<const TB>(a.gate, gate, a.ldg);
 #pragma unroll
         for (int j = 0; j < TEAM::NV; ++j) {
             if (t.full(j)) {
                 if (a.flags & F_PRE) load_raw(ph, j, t, hr), load_raw(pn, j, t, nr);
                 if (a.flags & F_READ_Y) load_raw(py, j, t, yr);
                 if (a.flags & F_STREAM_GRAD) load_raw(pd, j, t, dr);
-                if (GATE == G_ROW) load_raw(pg, j, t, gr);
+                if (ROW) load_raw(pg, j, t, gr);
             } else if (t.ends(j)) {
                 if (a.flags & F_PRE) load_part(ph, j, t, hr), load_part(pn, j, t, nr);
                 if (a.flags & F_READ_Y) load_part(py, j, t, yr);
                 if (a.flags & F_STREAM_GRAD) load_part(pd, j, t, dr);
-                if (GATE == G_ROW) load_part(pg, j, t, gr);
+                if (ROW) load_part(pg, j, t, gr);
             }
         }
     };
-    for (unsigned u = blockIdx.x; u < a.u.units; u += gridDim.x) {
-        const unsigned group = u / a.u.per_group, r1 = (group + 1) * a.u.span, step = a.u.per_group * t.rows;
-        const unsigned r0 = group * a.u.span + (u - group * a.u.per_group) * t.rows + t.row;
-        if (r0 < r1) fetch(r0);
+    const unsigned last = GATE == G_GROUP ? gridDim.x : a.u.units;
+    for (unsigned u = blockIdx.x; u < last; u += gridDim.x) {
+        const unsigned group = u / a.u.per_group, step = GATE == G_GROUP ? gridDim.x * t.rows : a.u.per_group * t.rows;
+        const unsigned r1 = GATE == G_GROUP ? a.u.units * a.u.span : (group + 1) * a.u.span;
+        unsigned gate = u * t.rows + t.row, left = a.u.span;         // G_GROUP: the row's gate row, rows that it has from here on
+        const unsigned r0 = GATE == G_GROUP ? gate * a.u.span : group * a.u.span + (u - group * a.u.per_group) * t.rows + t.row;
+        if (r0 < r1) fetch(r0, GATE == G_GROUP ? gate : r0);
         if (u == blockIdx.x) {
             load_gain(a.pw, t, pw, 1.f);
             load_gain(a.qw, t, qw, 1.f);
@@ -466,20 +491,23 @@ __global__ void __launch_bounds__(BLK ? 1024 : 256, BLK ? 4 : 3) rn_bwd_kernel(c
         sums.zero(S_PW), sums.zero(S_QW);
         if (SUM_T) sums.zero(S_PB);
         if (FULL) sums.zero(S_QB);
+        if (GATE == G_GROUP) sums.zero(S_GATE);
         float act[E];
         if (GATE == G_SHARED) {
             load_row(row_of<const TB>(a.gate, group, a.ldg), t, act);
 #pragma unroll
             for (int k = 0; k < E; ++k) act[k] = a.flags & F_SIGMOID ? sigmoid(act[k]) : act[k];
         }
-        for (unsigned r = r0; r < r1; r += step) {
+        unsigned next = 0;
+        for (unsigned r = r0; r < r1; r = next) {
             float hv[E], yv[E], T[E], g[E], gt[E];
             unpack(hr, t, hv);
             unpack(nr, t, g);
             unpack(yr, t, yv);
             unpack(dr, t, T);
-            if (GATE == G_ROW) unpack(gr, t, gt);
-            if (r + step < r1) fetch(r + step);
+            if (ROW) unpack(gr, t, gt);
+            next = GATE != G_GROUP ? r + step : left > 1 ? r + 1 : r + 1 + (step - 1) * a.u.span;
+            if (next < r1) fetch(next, GATE == G_GROUP ? gate + (left > 1 ? 0 : step) : next);
             float s[FULL ? 4 : 3];
             if (FULL && (a.flags & F_LAYER)) {
                 float m[2] = {sum_e(hv), sum_e(yv)};
@@ -512,7 +540,7 @@ __global__ void __launch_bounds__(BLK ? 1024 : 256, BLK ? 4 : 3) rn_bwd_kernel(c
             if (a.flags & F_BRANCH) {
 #pragma unroll
                 for (int k = 0; k < E; ++k) T[k] *= a.scale, yv[k] *= rs_y;
-                if (GATE == G_ROW) {
+                if (ROW) {
                     float dg[E], pb[E];
                     if (a.flags & F_POST) {
                         load_gain(a.pb, t, pb, 0.f);
@@ -528,7 +556,16 @@ __global__ void __launch_bounds__(BLK ? 1024 : 256, BLK ? 4 : 3) rn_bwd_kernel(c
                         dg[k] *= a.flags & F_SIGMOID ? ac * (1.f - ac) : 1.f;
                         T[k] *= ac;
                     }
-                    if (a.dgate) store_row(row_of<TB>(a.dgate, r, a.lddg), t, dg);
+                    if (GATE == G_ROW && a.dgate) store_row(row_of<TB>(a.dgate, r, a.lddg), t, dg);
+                    if (GATE == G_GROUP) {
+                        sums.add(S_GATE, dg);
+                        if (--left == 0) {
+                            sums.get(S_GATE, dg);
+                            if (a.dgate) store_row(row_of<TB>(a.dgate, gate, a.lddg), t, dg);
+                            sums.zero(S_GATE);
+                            left = a.u.span, gate += step;
+                        }
+                    }
                 }
                 if (SUM_T) sums.add(S_PB, T);
 #pragma unroll
@@ -574,20 +611,22 @@ __global__ void __launch_bounds__(BLK ? 1024 : 256, BLK ? 4 : 3) rn_bwd_kernel(c
             }
         }
         if (!BLK) __syncthreads();
-        float* part = a.part + (int64_t)blockIdx.x * a.nslot * a.pitch;
+        const int64_t off = (int64_t)blockIdx.x * a.step;
         const bool add = u != blockIdx.x;
         if constexpr (BLK) {
-            if (a.slot[0] >= 0) leave(S_PW, sums, t, lds, part + (int64_t)a.slot[0] * a.pitch, add);
-            if (a.slot[2] >= 0) leave(S_QW, sums, t, lds, part + (int64_t)a.slot[2] * a.pitch, add);
-            if (FULL && a.slot[1] >= 0) leave(S_PB, sums, t, lds, part + (int64_t)a.slot[1] * a.pitch, add);
-            if (FULL && a.slot[3] >= 0) leave(S_QB, sums, t, lds, part + (int64_t)a.slot[3] * a.pitch, add);
+            if (a.sums[0]) leave(S_PW, sums, t, lds, a.sums[0] + off, add);
+            if (a.sums[2]) leave(S_QW, sums, t, lds, a.sums[2] + off, add);
+            if (FULL && a.sums[1]) leave(S_PB, sums, t, lds, a.sums[1] + off, add);
+            if (FULL && a.sums[3]) leave(S_QB, sums, t, lds, a.sums[3] + off, add);
         } else {                     // all columns of all sums at once: few columns would leave most threads idle
-            for (int i = threadIdx.x; i < a.nslot * a.C; i += 256) {
-                const int slot = i / a.C, c = i - slot * a.C;
-                const int sum = slot == a.slot[0] ? S_PW : slot == a.slot[2] ? S_QW : slot == a.slot[1] ? S_PB : S_QB;
-                const float s = joined(sum, c, t, lds);
-                float* out = part + slot * a.pitch + c;
-                *out = add ? *out + s : s;
+            const int n = (FULL ? 4 : 2) * a.C, s = splits(n, t), k = threadIdx.x & ((1 << s) - 1);
+            for (int i = threadIdx.x >> s; i < n; i += blockDim.x >> s) {
+                const int sum = i / a.C, c = i - sum * a.C;
+                float* out = sum == S_PW ? a.sums[0] : sum == S_QW ? a.sums[2] : sum == S_PB ? a.sums[1] : a.sums[3];
+                if (!out) continue;
+                const float v = joined<NS>(sum, c, k, s, t, lds);
+                out += off + c;
+                if (k == 0) *out = add ? *out + v : v;
             }
             if (u + gridDim.x < a.u.units) __syncthreads();      // before the next unit's sums
         }
@@ -679,7 +718,7 @@ Shape shape_of(const sr_residual_norm_desc* d, int e) {
 
 struct Split {
     Units u = {1, 0, 1};
-    int blocks = 0;
+    int blocks = 0, resident = 0;    // workgroups; how many the GPU holds at once
     bool shared_gate = false;
 };
 
@@ -693,7 +732,7 @@ Split split_of(const sr_residual_norm_desc* d, const Shape& s, bool gate, unsign
     p.shared_gate = gate && rpg > 1;
     p.u.span = p.shared_gate ? rpg : (unsigned)d->rows;
     const int wg = s.threads / 64, fit = tight && wg > 4 ? waves / 4 / ((wg + 3) / 4) : waves / wg;
-    const int64_t groups = d->rows / p.u.span, resident = 256 * std::max(1, fit);
+    const int64_t groups = d->rows / p.u.span, resident = p.resident = 256 * std::max(1, fit);
     const int64_t most = (p.u.span + s.teams - 1) / s.teams;
     p.u.per_group = (unsigned)std::min(most, std::max<int64_t>(1, resident / groups));
     p.u.units = (unsigned)(groups * p.u.per_group);
@@ -729,8 +768,8 @@ void launch(const FwdArgs& a, bool blk, int gate, int blocks, int threads, hipSt
 
 template <typename TS, typename TB, int E, int VEC, bool BLK, bool TAIL, int GATE, bool FULL>
 void launch_bwd(const BwdArgs& a, int blocks, int threads, hipStream_t st) {
-    const int lds = (FULL ? 16 : GATE == G_SHARED ? 12 : 8) * E * threads + (BLK ? 1024 : 0);
-    if (BLK && lds > 64 * 1024)      // a launch may have 64 KiB unless the function says more
+    const int lds = 4 * ((FULL ? 4 : GATE == G_SHARED ? 3 : 2) + (GATE == G_GROUP)) * E * threads + (BLK ? 1024 : 0);
+    if (lds > 64 * 1024)             // a launch may have 64 KiB unless the function says more
         (void)hipFuncSetAttribute((const void*)rn_bwd_kernel<TS, TB, E, VEC, BLK, TAIL, GATE, FULL>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     rn_bwd_kernel<TS, TB, E, VEC, BLK, TAIL, GATE, FULL><<<blocks, threads, lds, st>>>(a);
 }
@@ -740,6 +779,9 @@ void launch_bwd(const BwdArgs& a, int gate, bool full, int blocks, int threads, 
     if (gate == G_NONE) {
         if constexpr (E == 8 || sizeof(TS) == 4)      // see bwd_plan
             full ? launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_NONE, true>(a, blocks, threads, st) : launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_NONE, false>(a, blocks, threads, st);
+    } else if (gate == G_GROUP) {
+        if constexpr (!BLK)
+            full ? launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_GROUP, true>(a, blocks, threads, st) : launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_GROUP, false>(a, blocks, threads, st);
     } else if (gate == G_ROW) full ? launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_ROW, true>(a, blocks, threads, st) : launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_ROW, false>(a, blocks, threads, st);
     else full ? launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_SHARED, true>(a, blocks, threads, st) : launch_bwd<TS, TB, E, VEC, BLK, TAIL, G_SHARED, false>(a, blocks, threads, st);
 }
@@ -757,6 +799,8 @@ struct BwdPlan {
     Shape s;
     Split p;
     size_t part, bytes;              // bytes of the partial sums, of everything
+    bool single;                     // one workgroup, which leaves the gradients themselves and needs no workspace
+    bool group;                      // G_GROUP
 };
 
 BwdPlan bwd_plan(const sr_residual_norm_desc* d, bool gate, unsigned rpg, bool full) {
@@ -772,7 +816,30 @@ BwdPlan bwd_plan(const sr_residual_norm_desc* d, bool gate, unsigned rpg, bool f
     const int wide = (C + 255) / 256;
     const bool e8 = d->stream_type == SR_T_F32 ? !gate && whole4 && wide > 8 && wide <= 12 : !gate || (whole8 && C > 1024);
     q.s = shape_of(d, C <= WAVE_C || C > 4096 || e8 ? 8 : 4);
+    // Few rows: one workgroup of up to 8 waves, and no launch that joins partial sums.  A call from Python takes 2.7 us less (of 17 to
+    // 22).  On the GPU a team's only row takes 3 us less, two one after the other -2.5 .. 1, a third 0 .. 2 us more, with a gate 2 .. 5.
+    const unsigned span = gate && rpg > 1 ? rpg : (unsigned)std::max<int64_t>(d->rows, 1);
+    const int threads = q.s.blk ? q.s.threads : q.s.tl ? 512 : 256, teams = q.s.blk ? 1 : threads >> q.s.tl;
+    const int64_t in_turn = d->rows / span * ((span + teams - 1) / teams);      // rows that a team then takes one after the other
+    q.group = false;
+    q.single = d->rows && in_turn <= (gate ? 2 : 3);
+    if (q.single) {
+        q.s.threads = threads, q.s.teams = teams;
+        q.p.u = {span, (unsigned)(d->rows / span), 1};
+        q.p.blocks = 1, q.p.shared_gate = gate && rpg > 1;
+        q.part = q.bytes = 0;
+        return q;
+    }
     q.p = split_of(d, q.s, gate, rpg, q.s.blk || (!full && !gate && whole8) ? 16 : 12, q.s.e == 8 || !whole4);
+    // Many gate rows, few rows each: a team takes a group by itself where that is a third of the rows one after the other, with 4 for
+    // the joining of a group's sums by a workgroup (62,499 x 64 bf16, 3 rows each: 25 us and not 172; 1,333,332 x 3: 41 and not 10,568;
+    // but 16 rows each, 62,496 x 64: 41 and not 55, 3 rows each, 1200 x 250: 14 and not 20)
+    if (q.p.shared_gate && !q.s.blk && q.p.u.per_group == 1) {
+        const int64_t groups = q.p.u.units, wgs = q.p.resident, teams = q.s.teams;
+        const int64_t by_team = (groups + wgs * teams - 1) / (wgs * teams) * span, shared = (groups + wgs - 1) / wgs * ((span + teams - 1) / teams + 4);
+        q.group = 3 * by_team <= shared;
+        if (q.group) q.p.blocks = (int)std::min(wgs, (groups + teams - 1) / teams);
+    }
     const size_t row = (size_t)round_up(d->channels, 4) * 4;
     q.part = round_up_sz((size_t)q.p.blocks * 4 * row);
     q.bytes = q.part + (q.p.shared_gate && q.p.u.per_group > 1 ? (size_t)q.p.u.units * row : 0);
@@ -945,18 +1012,21 @@ extern "C" int sr_op_residual_norm_bwd(int device, const sr_residual_norm_desc* 
     float* part = (float*)workspace;
     float* gpart = (float*)((char*)workspace + q.part);
     JoinArgs j = {part, {}, p.blocks, 0, {-1, -1, -1, -1}, C, round_up(C, 4), gpart, dgate, d->lddg, (int)p.u.per_group, d->branch_type};
+    float* sums[4];
     for (int i = 0; i < 4; ++i) {
-        j.out[i] = vec[i];
-        if (vec[i]) j.slot[i] = j.nslot++;
+        j.out[i] = sums[i] = vec[i];
+        if (!vec[i] || q.single) continue;
+        j.slot[i] = j.nslot++;
+        sums[i] = part + (int64_t)j.slot[i] * j.pitch;
     }
     if (d->rows) {
         const int flags = (dy ? F_BRANCH : 0) | (post ? F_POST : 0) | (pre ? F_PRE : 0) | (d->kind == SR_NORM_LAYER ? F_LAYER : 0) |
                           (d->gate_act == SR_GATE_SIGMOID ? F_SIGMOID : 0) | (dh ? F_STREAM_GRAD : 0) | (y ? F_READ_Y : 0);
         const BwdArgs a = {h, y, gate, dh, dn, post ? post_gain : nullptr, post ? post_bias : nullptr, pre ? pre_gain : nullptr, dx, dy, dgate,
-                           part, gpart, j.pitch, (int)d->ldh, (int)d->ldy, (int)d->ldg, (int)d->lddh, (int)d->lddn, (int)d->lddx, (int)d->lddy,
-                           (int)d->lddg, p.u, C, q.s.tl, flags, j.nslot, {j.slot[0], j.slot[1], j.slot[2], j.slot[3]}, d->scale, d->eps,
+                           {sums[0], sums[1], sums[2], sums[3]}, (int64_t)j.nslot * j.pitch, gpart, j.pitch, (int)d->ldh, (int)d->ldy, (int)d->ldg, (int)d->lddh, (int)d->lddn, (int)d->lddx, (int)d->lddy,
+                           (int)d->lddg, p.u, C, q.s.tl, flags, d->scale, d->eps,
                            1.f / (float)C};
-        const int gt = !gate ? G_NONE : p.shared_gate ? G_SHARED : G_ROW;
+        const int gt = !gate ? G_NONE : q.group ? G_GROUP : p.shared_gate ? G_SHARED : G_ROW;
 #define LAUNCH(TS, TB, VEC) launch<TS, TB, VEC>(a, q.s, gt, full, p.blocks, st)
         RN_TYPES(LAUNCH);
 #undef LAUNCH

@@ -1129,7 +1129,7 @@ def residual_norm_bwd(h, y=None, dh=None, dn=None, gate=None, post_gain=None, po
         size = C.c_size_t()
         _check(lib().sr_op_residual_norm_bwd_workspace(d, gate is not None, C.byref(size)))
         need = _bwd_bytes[key] = size.value
-    ws = _torch.empty(need, dtype=_torch.uint8, device=h.device)
+    ws = _torch.empty(need, dtype=_torch.uint8, device=h.device) if need else None
     out = [_vector_like(post_gain, C_, h) if post else None, _vector_like(post_gain, C_, h) if post and bias_grads else None,
            _vector_like(pre_gain, C_, h) if pre else None, _vector_like(pre_gain, C_, h) if pre and bias_grads else None]
     rc = lib().sr_op_residual_norm_bwd(dev, d, h.data_ptr(), None if y is None else y.data_ptr(), None if gate is None else gate.data_ptr(),
@@ -1137,7 +1137,7 @@ def residual_norm_bwd(h, y=None, dh=None, dn=None, gate=None, post_gain=None, po
                                        _vector(pre_gain, "pre_gain", C_, dev), None if dh is None else dh.data_ptr(),
                                        None if dn is None else dn.data_ptr(), dx.data_ptr(), None if dy is None else dy.data_ptr(),
                                        None if dgate is None else dgate.data_ptr(), *[None if v is None else v.data_ptr() for v in out],
-                                       ws.data_ptr(), need, _current_stream(dev))
+                                       None if ws is None else ws.data_ptr(), need, _current_stream(dev))
     if rc:
         _check(rc)
     return ResidualNormGrads(dx, dy, dgate, *out)

@@ -204,6 +204,32 @@ def test_backward_many_rows(sh, lead, C, gate):
     check_bwd(sh, case(6, lead, C, BF16, BF16, "element"), "both", "rms", "linear")
 
 
+@pytest.mark.parametrize("C", [1, 3, 7, 9, 13, 16, 33, 64, 65, 130, 257, 511])
+@pytest.mark.parametrize("lead,gate", [((6001,), None), ((6002,), "element"), ((3000, 2), 3000), ((2401, 3), 2401), ((450, 17), 450), ((70, 90), 70),
+                                       ((2, 3001), 2)])
+def test_backward_rows_within_a_wave(sh, C, lead, gate):
+    """More rows than one workgroup takes, of few channels, and gate rows for two rows and for thousands: a team's own, a workgroup's,
+    several workgroups'."""
+    i = C + lead[-1]
+    ts, tb = TYPES[i % 5]
+    check_bwd(sh, case(i, lead, C, ts, tb, gate), "both", ["rms", "layer"][i // 2 % 2], "sigmoid")
+    check_bwd(sh, case(i, lead, C, F32, F32, gate, bias=False), ["both", "post", "pre"][i % 3], "rms", "linear")
+
+
+@pytest.mark.parametrize("C,teams", [(5, 256), (16, 256), (64, 64), (250, 16), (500, 8), (700, 1), (4100, 1)])
+@pytest.mark.parametrize("gate", [None, "element", 1, 2])
+def test_backward_around_one_workgroup(sh, C, teams, gate):
+    """Rows up to what one workgroup takes, which leaves the gradients itself, and one more."""
+    for rows in (1, 2, teams, teams + 1, 2 * teams, 2 * teams + 2, 3 * teams, 3 * teams + 1):
+        if gate == 2 and rows % 2:
+            continue
+        c = case(rows, (rows,), C, BF16, BF16, gate)
+        a = check_bwd(sh, c, "both", "layer", "sigmoid")
+        b = check_bwd(sh, c, "both", "layer", "sigmoid")
+        for p, q in zip(a, b):
+            assert (p is None and q is None) or torch.equal(p, q)
+
+
 @pytest.mark.parametrize("ts,tb", [(F32, F32), (BF16, BF16), (F32, F16)])
 def test_rows_of_a_wider_matrix(sh, ts, tb):
     """Pitches, odd starts, outputs beside inputs in one buffer; what lies between the rows stays as it was."""

@@ -82,15 +82,19 @@ def test_bad_calls_forward():
 
 def test_bad_calls_backward():
     assert backward(None)[0] == -1
-    for kw in (dict(h=None), dict(dn=None), dict(dx=None), dict(y=None), dict(dy=None), dict(dgate=9 * P), dict(ws=None), dict(ws=16 * P + 8),
-               dict(size=16)):
+    for kw in (dict(h=None), dict(dn=None), dict(dx=None), dict(y=None), dict(dy=None), dict(dgate=9 * P)):
         assert backward(desc(), **kw)[0] == -1, kw
+    many = desc(rows=4000)
+    assert backward(many)[0] == -4
+    for kw in (dict(ws=None), dict(ws=16 * P + 8), dict(size=16), dict(ws=5 * P), dict(ws=7 * P), dict(gains=(None, None, 16 * P))):
+        assert backward(many, **kw)[0] == -1, kw
+    assert backward(desc(), ws=None, size=0)[0] == -4                    # a few rows: no workspace
     assert backward(desc(), dh=None)[0] == -4
     assert backward(desc(norms=1), dh=None, vec=(None,) * 4)[0] == -1
     assert backward(desc(norms=1), vec=(7 * P, None, 8 * P, None))[0] == -1      # no pre norm, so no gradient of its gain
     assert backward(desc(norms=2), vec=(None, 7 * P, None, None))[0] == -1
-    for kw in (dict(dx=P + 4), dict(dy=5 * P), dict(dx=7 * P - 4), dict(vec=(7 * P, 7 * P + 32, None, None)), dict(ws=5 * P), dict(ws=7 * P),
-               dict(gains=(5 * P, None, None)), dict(gains=(None, None, 16 * P))):
+    for kw in (dict(dx=P + 4), dict(dy=5 * P), dict(dx=7 * P - 4), dict(vec=(7 * P, 7 * P + 32, None, None)),
+               dict(gains=(5 * P, None, None)), dict(gains=(None, None, 8 * P))):
         rc, msg = backward(desc(), **kw)
         assert rc == -1 and "overlaps" in msg, kw
     assert backward(desc(), dx=P, dy=2 * P)[0] == -4
