@@ -636,7 +636,9 @@ __global__ void __launch_bounds__(BLK ? 1024 : 512, BLK ? 4 : 3) rn_bwd_kernel(c
 // The partial sums of a backward pass joined in a fixed order: 4 columns a thread, LC threads side by side, 1024 / LC slices of the
 // partial sums.  16 threads side by side read 256 bytes at a time (24 MB of sums for 6000 channels: 7.0 us, with 4 threads 12.9), 4
 // give four times the workgroups where the columns are few (2 x 771: 5.4 us instead of 12.4).  blockIdx.y < 4: the gradient of that
-// gain or bias over the workgroups; beyond: gate row blockIdx.y - 4 over its units.
+// gain or bias over the workgroups; beyond: gate row blockIdx.y - 4 over its units, or, where these are few, a thread for 4 columns of
+// any gate row (4000 x 1000 bf16 with 500 gate rows of 2 units: 26 us and not 45 for the call; 8192 x 4096 with 16 rows of 32 units: 114 and not 109).
+constexpr int FEW_UNITS = 16;
 struct JoinArgs {
     const float* part;
     float* out[4];
@@ -644,8 +646,20 @@ struct JoinArgs {
     const float* gpart;
     void* dgate;
     int64_t lddg;
-    int per_group, branch_type;
+    int per_group, branch_type, gates;
 };
+
+// 4 columns from c on of a row of dgate
+__device__ __forceinline__ void store_gate(const JoinArgs& a, int64_t row, int c, const float (&s)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (c + k >= a.C) break;
+        const int64_t i = row * a.lddg + c + k;
+        if (a.branch_type == SR_T_F32) ((float*)a.dgate)[i] = s[k];
+        else if (a.branch_type == SR_T_BF16) ((bf16_t*)a.dgate)[i] = (bf16_t)s[k];
+        else ((f16_t*)a.dgate)[i] = (f16_t)s[k];
+    }
+}
 
 template <int LC>
 __global__ void __launch_bounds__(1024) rn_join_kernel(const JoinArgs a) {
@@ -653,6 +667,20 @@ __global__ void __launch_bounds__(1024) rn_join_kernel(const JoinArgs a) {
     __shared__ float4 sm[SL * LC];
     const int cl = threadIdx.x % LC, sl = threadIdx.x / LC, c = (blockIdx.x * LC + cl) * 4, job = blockIdx.y;
     const bool gate = job >= 4;
+    if (gate && a.per_group <= FEW_UNITS) {
+        const int64_t q = a.pitch / 4, i = ((int64_t)(job - 4) * gridDim.x + blockIdx.x) * 1024 + threadIdx.x, row = i / q;
+        if (row >= a.gates) return;
+        const int at = (int)(i - row * q) * 4;
+        const float* p = a.gpart + row * a.per_group * a.pitch + at;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int u = 0; u < a.per_group; ++u) {
+            const float4 v = *reinterpret_cast<const float4*>(p + (int64_t)u * a.pitch);
+            s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
+        }
+        store_gate(a, row, at, s);
+        return;
+    }
     if (!gate && !a.out[job]) return;
     const float* p = gate ? a.gpart + (int64_t)(job - 4) * a.per_group * a.pitch : a.part + (int64_t)a.slot[job] * a.pitch;
     const int64_t step = gate ? a.pitch : (int64_t)a.nslot * a.pitch;
@@ -682,18 +710,13 @@ __global__ void __launch_bounds__(1024) rn_join_kernel(const JoinArgs a) {
         __syncthreads();
     }
     if (sl) return;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        if (c + k >= a.C) break;
-        if (!gate)
-            a.out[job][c + k] = s[k];
-        else if (a.branch_type == SR_T_F32)
-            ((float*)a.dgate)[(job - 4) * a.lddg + c + k] = s[k];
-        else if (a.branch_type == SR_T_BF16)
-            ((bf16_t*)a.dgate)[(job - 4) * a.lddg + c + k] = (bf16_t)s[k];
-        else
-            ((f16_t*)a.dgate)[(job - 4) * a.lddg + c + k] = (f16_t)s[k];
+    if (gate) {
+        store_gate(a, job - 4, c, s);
+        return;
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (c + k < a.C) a.out[job][c + k] = s[k];
 }
 
 // ------------------------------------------------------------------------------------------------- host
@@ -1035,7 +1058,10 @@ extern "C" int sr_op_residual_norm_bwd(int device, const sr_residual_norm_desc* 
     const unsigned gates = dgate && p.shared_gate && p.u.per_group > 1 ? (unsigned)(d->rows / rpg) : 0;
     if (e == hipSuccess && (j.nslot || gates)) {
         const bool wide = (int64_t)(j.nslot + gates) * C >= 2048;
-        const dim3 grid((C + (wide ? 63 : 15)) / (wide ? 64 : 16), 4 + gates);
+        const unsigned across = (C + (wide ? 63 : 15)) / (wide ? 64 : 16);
+        const int64_t quads = (int64_t)gates * (j.pitch / 4);
+        j.gates = (int)gates;
+        const dim3 grid(across, 4 + (p.u.per_group <= FEW_UNITS ? (unsigned)((quads + across * 1024 - 1) / (across * 1024)) : gates));
         if (wide) rn_join_kernel<16><<<grid, 1024, 0, st>>>(j);
         else rn_join_kernel<4><<<grid, 1024, 0, st>>>(j);
         e = hipGetLastError();

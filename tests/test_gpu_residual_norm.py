@@ -196,7 +196,8 @@ def test_backward(sh, C, types):
 
 
 @pytest.mark.parametrize("lead,C,gate", [((40, 640), 64, 40), ((7, 1000), 48, 7), ((1500, 3), 64, 1500), ((3000,), 520, 1), ((2, 1300), 1030, 2), ((2100, 2), 521, 2100),
-                                         ((600, 2), 4100, 600), ((2, 4, 300), 250, 2)])
+                                         ((600, 2), 4100, 600), ((2, 4, 300), 250, 2), ((500, 8), 1001, 500), ((60, 40), 4096, 60),
+                                         ((9, 3000), 20, 9)])
 def test_backward_many_rows(sh, lead, C, gate):
     """Several workgroups to a gate row, several gate rows to a workgroup (which then adds to its partial sums), gate rows that are
     whole in one."""
