@@ -637,7 +637,8 @@ __global__ void __launch_bounds__(BLK ? 1024 : 512, BLK ? 4 : 3) rn_bwd_kernel(c
 // partial sums.  16 threads side by side read 256 bytes at a time (24 MB of sums for 6000 channels: 7.0 us, with 4 threads 12.9), 4
 // give four times the workgroups where the columns are few (2 x 771: 5.4 us instead of 12.4).  blockIdx.y < 4: the gradient of that
 // gain or bias over the workgroups; beyond: gate row blockIdx.y - 4 over its units, or, where these are few, a thread for 4 columns of
-// any gate row (4000 x 1000 bf16 with 500 gate rows of 2 units: 26 us and not 45 for the call; 8192 x 4096 with 16 rows of 32 units: 114 and not 109).
+// any gate row (4000 x 1000 bf16 with 500 gate rows of 2 units: 26 us and not 45 for the call; 8192 x 4096 with 16 rows of 32 units:
+// 114 and not 109).
 constexpr int FEW_UNITS = 16;
 struct JoinArgs {
     const float* part;
