@@ -330,6 +330,22 @@ def test_infinities_and_nan_stay_in_their_row(sh):
         assert got.pre_gain.isnan().any()
 
 
+def test_nan_stays_in_its_gate_row(sh):
+    """Gate rows of 2, 50 and 2000 positions: a team's own, a workgroup's, several workgroups'."""
+    for rows, G, C in ((6000, 3000, 24), (6000, 120, 40), (6000, 3, 64), (4000, 2000, 600)):
+        c = case(14, (rows,), C, F32, BF16, G)
+        kw = dict(gate=c["gate"], post_gain=c["post_gain"], pre_gain=c["pre_gain"], kind="layer")
+        want = sh.residual_norm_bwd(c["x"], c["y"], c["dh"], c["dn"], **kw)
+        dn = c["dn"].clone()
+        dn[rows // G] = float("nan")             # the first position of gate row 1
+        got = sh.residual_norm_bwd(c["x"], c["y"], c["dh"], dn, **kw)
+        keep = torch.arange(G, device="cuda") != 1
+        assert torch.equal(got.dgate[keep], want.dgate[keep]) and got.dgate[1].isnan().all()
+        keep = torch.arange(rows, device="cuda") != rows // G
+        assert torch.equal(got.dx[keep], want.dx[keep]) and torch.equal(got.dy[keep], want.dy[keep])
+        assert got.dx[~keep].isnan().all() and got.pre_gain.isnan().all()
+
+
 def test_against_differences(sh):
     """d/dt of <h, dh> + <n, dn> along a direction in all inputs, by central differences D of the forward kernel, extrapolated:
     (4 D(t / 2) - D(t)) / 3 is off by t^4 / 480 of the fifth derivative (t = 2^-6: 1e-10) and by rounding: 5760 terms of about 2,
@@ -394,6 +410,30 @@ def test_captured_and_replayed(sh):
         torch.cuda.synchronize()
         for a, b in zip(out, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows,G,C", [(5, 1, 48), (6000, 3000, 24), (2000, 250, 1000)])
+def test_captured_twice_with_other_work_between(sh, rows, G, C):
+    """Two graphs of the same call, replayed in turn with eager calls: each has a workspace of its own, or none."""
+    c = case(13, (rows,), C, F32, F32, G)
+    kw = dict(gate=c["gate"], post_gain=c["post_gain"], pre_gain=c["pre_gain"], gate_act="sigmoid")
+    call = lambda dn: [v for v in sh.residual_norm_bwd(c["x"], c["y"], c["dh"], dn, **kw) if v is not None]
+    other = 2 * c["dn"]
+    want = call(c["dn"]), call(other)
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for g, dn in zip(graphs, (c["dn"], other)):
+        with torch.cuda.graph(g):
+            outs.append(call(dn))
+    for i in range(3):
+        for o in outs[0] + outs[1]:
+            o.fill_(7.0)
+        graphs[i % 2].replay()
+        graphs[1 - i % 2].replay()
+        call(other)
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(o, w))
 
 
 def test_positions_behind_2_31_elements(sh):
