@@ -430,7 +430,7 @@ enum sr_gate_act { SR_GATE_LINEAR = 0, SR_GATE_SIGMOID = 1 };
  * sr_op_residual_norm_bwd: from h (needed with SR_NORM_PRE), y (with SR_NORM_POST or a gate), dh = the gradient that reaches h
  *   through the stream (NULL: none; needed without SR_NORM_PRE) and dn (with SR_NORM_PRE) to dx = the whole gradient of h, dy (NULL:
  *   there is no branch), dgate (NULL: not wanted) and the vectors that are not NULL.  Row statistics are taken again from h and y.
- *   dx, dy may be h, y, dh or dn (same type and pitch).  rows == 0 zeroes the vectors.  `workspace`:
+ *   dx, dy may be h, y, dh or dn (same type and pitch).  rows == 0 zeroes the vectors (a gate has no rows then).  `workspace`:
  *   sr_op_residual_norm_bwd_workspace bytes (gate: whether there is one; 0 where there are few rows: then it may be NULL),
  *   16-byte aligned. */
 typedef struct sr_residual_norm_desc {

@@ -1117,7 +1117,9 @@ def residual_norm_bwd(h, y=None, dh=None, dn=None, gate=None, post_gain=None, po
             lddy = _pitch(dy, "dy", shape, bt, dev)
     elif dy is not None:
         raise ValueError("dy without a branch")
-    dgate = like.new_empty(gate.shape) if gate is not None else None
+    dgate = None
+    if gate is not None:             # gate rows of no positions: the sum over none, which no launch would write
+        dgate = like.new_empty(gate.shape) if rows else like.new_zeros(gate.shape)
     d = _pack_block(rows, rpg, 0, ldy, ldg, ldh, 0, lddh, lddn, lddx, lddy, C_, C_, st, _type_of(bt, "y"), _KINDS[kind], mask,
                     _GATES[gate_act], scale, eps)
     # the workspace goes by these alone
