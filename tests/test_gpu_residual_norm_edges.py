@@ -1,10 +1,16 @@
-"""residual_norm and residual_norm_bwd where inputs are at an edge."""
+"""residual_norm and residual_norm_bwd where inputs are at an edge, and without the gradients of biases.
+
+Formulas, magnitudes and tolerances are those of test_gpu_residual_norm.py: eps_T / 2 of the value, plus K * 2^-24 of the formula with
+every term replaced by its magnitude.  K = 256 for what a row's own values give; a sum over rows adds its chain, which for the
+shapes here is at most 25 rows of a team, 8 slices and 18 levels of joining: 51 roundings more, K = 320."""
 import pytest
 import torch
 
-from test_gpu_residual_norm import BF16, F16, F32, randn
+from test_gpu_residual_norm import BF16, F16, F32, TYPES, case, expect_bwd, randn, within
 
 pytestmark = pytest.mark.gpu
+
+K = 320
 
 
 @pytest.fixture(scope="module")
@@ -28,3 +34,48 @@ def test_gate_gradient_of_no_rows_is_zero(sh, dt, lead, gate):
         got = sh.residual_norm_bwd(x, x, x, x, gate=g, bias_grads=True)
         assert got.dgate.shape == g.shape and got.dgate.dtype == dt and not got.dgate.any()
         assert got.dx.shape == got.dy.shape == x.shape and not any(bool(v.any()) for v in got[3:])
+
+
+def check_gains_only(sh, c, norms, act="sigmoid", scale=0.7, eps=1e-5):
+    """An rms norm without the gradients of biases: kernels of their own."""
+    want = {k: v for k, v in expect_bwd(c, norms, "rms", act, scale, eps).items() if not k.endswith("bias")}
+    got = sh.residual_norm_bwd(c["x"], c["y"], c["dh"], c["dn"] if norms != "post" else None, gate=c["gate"], post_gain=c["post_gain"],
+                               post_bias=c["post_bias"], pre_gain=c["pre_gain"], norms=norms, kind="rms", gate_act=act, scale=scale, eps=eps)
+    for name, v in got._asdict().items():
+        assert (v is None) == (name not in want), name
+        if v is not None:
+            ref, mag = want[name]
+            within(v.reshape(ref.shape), ref, mag, K, name)
+
+
+@pytest.mark.parametrize("C", [1, 3, 8, 33, 64, 65, 250, 256, 511, 512, 513, 520, 771, 1000, 1541, 2048, 4095, 4097, 5000, 8191, 8192])
+@pytest.mark.parametrize("types", range(5))
+def test_gains_only(sh, C, types):
+    """Few rows (one workgroup) and more, no gate, a gate for each element, one gate row, a gate row for half of the rows."""
+    ts, tb = TYPES[types]
+    for i, (rows, gate) in enumerate([(2, None), (2, "element"), (700, None), (700, "element"), (700, 1), (700, 2)]):
+        j = i + C + types
+        check_gains_only(sh, case(j, (rows,), C, ts, tb, gate, ["both", "post", "pre"][j % 3], bias=j % 2 == 0, gains=j % 5 != 0), ["both", "post", "pre"][j % 3],
+                         ["linear", "sigmoid"][j // 2 % 2])
+
+
+@pytest.mark.parametrize("C", [1, 7, 16, 65, 130, 257, 511])
+@pytest.mark.parametrize("lead,gate", [((6001,), None), ((6002,), "element"), ((3000, 2), 3000), ((2001, 3), 2001), ((350, 17), 350), ((2, 3001), 2)])
+def test_gains_only_rows_within_a_wave(sh, C, lead, gate):
+    """Gate rows of a team, of a workgroup, of several workgroups."""
+    for ts, tb in ((F32, F32), (BF16, BF16), (F32, F16)):
+        check_gains_only(sh, case(C, lead, C, ts, tb, gate), "both")
+
+
+@pytest.mark.parametrize("C", [2048, 2056, 2060, 2304, 2600, 3060, 3080, 3300])
+def test_gains_only_fp32_rows_of_eight_to_thirteen_waves(sh, C):
+    """Without a gate a lane has 8 elements of these rows, or 4."""
+    for tb in (F32, BF16):
+        check_gains_only(sh, case(C, (600,), C, F32, tb, None), "both")
+
+
+@pytest.mark.parametrize("lead,C,gate", [((1500, 3), 520, 1500), ((600, 2), 4100, 600), ((500, 8), 1001, 500), ((60, 40), 4096, 60), ((2, 1300), 1030, 2)])
+def test_gains_only_long_rows_that_share_a_gate(sh, lead, C, gate):
+    """Several gate rows to a workgroup, a gate row to one or to several."""
+    for ts, tb in ((F32, F32), (BF16, BF16)):
+        check_gains_only(sh, case(3, lead, C, ts, tb, gate), "both")
