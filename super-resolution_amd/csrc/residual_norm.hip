@@ -242,6 +242,9 @@ __device__ __forceinline__ float dot_e(const float (&a)[E], const float (&b)[E])
     return s + u;
 }
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + expf(-g)); }   // rcp: 1 ulp
+// its slope s (1 - s), where s = sigmoid(g).  1 - s is exp(-g) s as well, which keeps its precision where s is close to 1 (from g = 17
+// on the difference is 0); far below 0 exp(-g) is infinite, but the difference exact to a rounding
+__device__ __forceinline__ float sigmoid_slope(float g, float s) { return s * (g > 0.f ? expf(-g) * s : 1.f - s); }
 
 // one row of anything, 0 behind it
 template <typename T, typename TEAM>
@@ -442,6 +445,12 @@ __device__ __forceinline__ void leave(int i, const Sums<TEAM::E, NS>& sums, cons
     }
 }
 
+// The places in LDS that a backward pass has: its sums over rows; G_GROUP's sum for dgate; the slopes of a sigmoid gate that a unit's
+// rows share.  Taken from the gate again at the end of the unit the slopes cost 0.4 us a unit (62,496 x 64 bf16, 16 rows each: 42 us and
+// not 40); rows of a workgroup do that all the same, 1024 lanes leave no room for them.
+template <int GATE, bool FULL, bool BLK>
+constexpr int bwd_sums() { return (FULL ? 4 : GATE == G_SHARED ? 3 : 2) + (GATE == G_GROUP || (GATE == G_SHARED && !BLK)); }
+
 // Rows in turn like the forward pass (8192 x 4096 bf16: 80.5 us, 5.0 TB/s; 163,840 x 64 fp32 with a gate an image: 50 us, 5.0 TB/s).
 // FULL: layer norms or gradients of biases; without, only what rms norms with gains need is in registers.  The sums over rows are
 // those of a unit; a workgroup with several units adds them up in its partial sums.  With a gate that a unit shares they are
@@ -450,7 +459,7 @@ template <typename TS, typename TB, int E, int VEC, bool BLK, bool TAIL, int GAT
 __global__ void __launch_bounds__(BLK ? 1024 : 512, BLK ? 4 : 3) rn_bwd_kernel(const BwdArgs a) {
     extern __shared__ float lds[];   // the sums, then BLK's [2][16][E] floats
     constexpr bool ROW = GATE == G_ROW || GATE == G_GROUP;
-    constexpr int NS = (FULL ? 4 : GATE == G_SHARED ? 3 : 2) + (GATE == G_GROUP);
+    constexpr int NS = bwd_sums<GATE, FULL, BLK>();
     enum { S_PW, S_QW, S_PB, S_QB, S_GATE = NS - 1 };
     using TEAM = Team<E, VEC, BLK, TAIL>;
     TEAM t(a.tl, a.C, lds + NS * E * blockDim.x);
@@ -495,8 +504,18 @@ __global__ void __launch_bounds__(BLK ? 1024 : 512, BLK ? 4 : 3) rn_bwd_kernel(c
         float act[E];
         if (GATE == G_SHARED) {
             load_row(row_of<const TB>(a.gate, group, a.ldg), t, act);
+            if (!BLK && a.flags & F_SIGMOID) {
+                float slope[E];
 #pragma unroll
-            for (int k = 0; k < E; ++k) act[k] = a.flags & F_SIGMOID ? sigmoid(act[k]) : act[k];
+                for (int k = 0; k < E; ++k) {
+                    const float ac = sigmoid(act[k]);
+                    slope[k] = sigmoid_slope(act[k], ac), act[k] = ac;
+                }
+                sums.set(S_GATE, slope);
+            } else {
+#pragma unroll
+                for (int k = 0; k < E; ++k) act[k] = a.flags & F_SIGMOID ? sigmoid(act[k]) : act[k];
+            }
         }
         unsigned next = 0;
         for (unsigned r = r0; r < r1; r = next) {
@@ -553,7 +572,7 @@ __global__ void __launch_bounds__(BLK ? 1024 : 512, BLK ? 4 : 3) rn_bwd_kernel(c
 #pragma unroll
                     for (int k = 0; k < E; ++k) {
                         const float ac = a.flags & F_SIGMOID ? sigmoid(gt[k]) : gt[k];
-                        dg[k] *= a.flags & F_SIGMOID ? ac * (1.f - ac) : 1.f;
+                        dg[k] *= a.flags & F_SIGMOID ? sigmoid_slope(gt[k], ac) : 1.f;
                         T[k] *= ac;
                     }
                     if (GATE == G_ROW && a.dgate) store_row(row_of<TB>(a.dgate, r, a.lddg), t, dg);
@@ -594,10 +613,21 @@ __global__ void __launch_bounds__(BLK ? 1024 : 512, BLK ? 4 : 3) rn_bwd_kernel(c
             load_gain(a.pb, t, pb, 0.f);
             // S_PB's place takes dgate until it is out
 #pragma unroll
-            for (int k = 0; k < E; ++k) {
-                pb[k] = (a.flags & F_POST ? pw[k] * v[k] + pb[k] * w[k] : v[k]) * (a.flags & F_SIGMOID ? act[k] * (1.f - act[k]) : 1.f);
-                v[k] *= act[k], w[k] *= act[k];
+            for (int k = 0; k < E; ++k) pb[k] = a.flags & F_POST ? pw[k] * v[k] + pb[k] * w[k] : v[k];
+            if (a.flags & F_SIGMOID && a.dgate) {
+                float slope[E];
+                if constexpr (BLK) {
+                    load_row(row_of<const TB>(a.gate, group, a.ldg), t, slope);
+#pragma unroll
+                    for (int k = 0; k < E; ++k) slope[k] = sigmoid_slope(slope[k], act[k]);
+                } else {
+                    sums.get(S_GATE, slope);
+                }
+#pragma unroll
+                for (int k = 0; k < E; ++k) pb[k] *= slope[k];
             }
+#pragma unroll
+            for (int k = 0; k < E; ++k) v[k] *= act[k], w[k] *= act[k];
             sums.set(S_PW, v);
             sums.set(S_PB, pb);
             if (!BLK) __syncthreads();
@@ -792,7 +822,7 @@ void launch(const FwdArgs& a, bool blk, int gate, int blocks, int threads, hipSt
 
 template <typename TS, typename TB, int E, int VEC, bool BLK, bool TAIL, int GATE, bool FULL>
 void launch_bwd(const BwdArgs& a, int blocks, int threads, hipStream_t st) {
-    const int lds = 4 * ((FULL ? 4 : GATE == G_SHARED ? 3 : 2) + (GATE == G_GROUP)) * E * threads + (BLK ? 1024 : 0);
+    const int lds = 4 * bwd_sums<GATE, FULL, BLK>() * E * threads + (BLK ? 1024 : 0);
     if (lds > 64 * 1024)             // a launch may have 64 KiB unless the function says more
         (void)hipFuncSetAttribute((const void*)rn_bwd_kernel<TS, TB, E, VEC, BLK, TAIL, GATE, FULL>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     rn_bwd_kernel<TS, TB, E, VEC, BLK, TAIL, GATE, FULL><<<blocks, threads, lds, st>>>(a);

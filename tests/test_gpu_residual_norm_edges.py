@@ -6,6 +6,7 @@ shapes here is at most 25 rows of a team, 8 slices and 18 levels of joining: 51 
 import pytest
 import torch
 
+import test_gpu_residual_norm as base
 from test_gpu_residual_norm import BF16, F16, F32, TYPES, case, expect_bwd, randn, within
 
 pytestmark = pytest.mark.gpu
@@ -79,3 +80,31 @@ def test_gains_only_long_rows_that_share_a_gate(sh, lead, C, gate):
     """Several gate rows to a workgroup, a gate row to one or to several."""
     for ts, tb in ((F32, F32), (BF16, BF16)):
         check_gains_only(sh, case(3, lead, C, ts, tb, gate), "both")
+
+
+def far_gates(c, rows, C, act):
+    """gate_of of test_gpu_residual_norm.py without the cancellation of 1 - sigmoid(g)."""
+    g = c["gate"].double().reshape(-1, C)
+    g = g.repeat_interleave(rows // g.shape[0], 0)
+    return torch.sigmoid(g), torch.sigmoid(g) * torch.sigmoid(-g)
+
+
+@pytest.mark.parametrize("C", [24, 65, 600, 4100])
+@pytest.mark.parametrize("lead,gate", [((5,), "element"), ((900,), "element"), ((4, 2), 4), ((1500, 2), 1500), ((3000, 2), 3000), ((90, 40), 90), ((2, 700), 2)])
+def test_gradient_of_far_gates(sh, monkeypatch, C, lead, gate):
+    """The slope of a sigmoid far out is exp(-|g|), however close to 1 the sigmoid itself is: the gradient keeps its precision there.
+    The slope is made of an exponential (2 ulp), a reciprocal (1 ulp), a sum and two products, well inside of K."""
+    monkeypatch.setattr(base, "gate_of", far_gates)
+    for ts, tb in ((F32, F32), (F32, BF16)):
+        c = case(7, lead, C, ts, tb, gate)
+        steps = torch.tensor([0.0, 2.0, 5.0, 8.0, 12.0, 16.0, 16.625, 17.0, 20.0, 40.0, 80.0], device="cuda")
+        g = steps.repeat_interleave(2) * torch.tensor([1.0, -1.0], device="cuda").repeat(len(steps))
+        c["gate"] = g.repeat(c["gate"].numel() // len(g) + 1)[:c["gate"].numel()].reshape(c["gate"].shape).to(tb)
+        for kind, bias in (("rms", False), ("layer", True)):
+            want = expect_bwd(c, "both", kind, "sigmoid", 0.7, 1e-5)
+            got = sh.residual_norm_bwd(c["x"], c["y"], c["dh"], c["dn"], gate=c["gate"], post_gain=c["post_gain"], post_bias=c["post_bias"],
+                                       pre_gain=c["pre_gain"], kind=kind, gate_act="sigmoid", scale=0.7, eps=1e-5, bias_grads=bias)
+            for name, v in got._asdict().items():
+                if v is not None:
+                    ref, mag = want[name]
+                    within(v.reshape(ref.shape), ref, mag, K, name)
