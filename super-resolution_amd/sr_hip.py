@@ -948,9 +948,18 @@ def _on(stream, device):
     return _torch.cuda.stream(_torch.cuda.ExternalStream(int(stream), device=device))
 
 
+def _no_graph(what):
+    # without this a module built on these calls would train without the gradients and say nothing
+    if _torch.is_grad_enabled():
+        raise ValueError(f"{what} requires grad, and this call builds no graph: make it under torch.no_grad() or in the forward of a "
+                         f"torch.autograd.Function, with residual_norm_bwd in its backward")
+
+
 def _pitch(t, what, shape, dtype, dev):
     """Elements between the rows of t (..., C), as many as `shape` has, seen as a matrix; the checks every tensor of a call goes
     through.  dev: the device's number."""
+    if t.requires_grad:
+        _no_graph(what)
     if t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous():
         return shape[-1]
     C_ = shape[-1]
@@ -973,6 +982,8 @@ def _pitch(t, what, shape, dtype, dev):
 def _vector(t, what, C_, dev):
     if t is None:
         return None
+    if t.requires_grad:
+        _no_graph(what)
     if t.dtype is not _torch.float32 or t.get_device() != dev or t.dim() != 1 or t.numel() != C_ or not t.is_contiguous():
         raise ValueError(f"{what}: expected a contiguous float32 vector of {C_} on cuda:{dev}")
     return t.data_ptr()
@@ -1027,7 +1038,8 @@ def residual_norm(x, y=None, gate=None, post_gain=None, post_bias=None, pre_gain
     them in a row share one: (B, C), or (B, 1, 1, C), gates the channels of each image of an NHWC batch.  norms 'both', 'post' or
     'pre', kind 'rms' or 'layer', gains and biases float32.  Without y: n = pre(x) in branch_dtype (default x's), and h is x.  h, n:
     tensors to write (h may be x, n may be y), default new ones.  Returns (h, n), n None with norms 'post'.  Runs on `stream` (a
-    hipStream_t as int), default torch's current one."""
+    hipStream_t as int), default torch's current one.  Builds no graph: while torch records gradients, tensors that require them are
+    refused."""
     if stream is not None:
         with _on(stream, x.device):
             return residual_norm(x, y, gate, post_gain, post_bias, pre_gain, pre_bias, norms, kind, gate_act, scale, eps, branch_dtype, h, n)
