@@ -908,6 +908,7 @@ _GATES = {"linear": 0, "sigmoid": 1}
 _torch = None
 _torch_types = None
 _current_stream = None
+_count_change = None
 _bwd_bytes = {}      # bytes of workspace of the backward calls made so far
 _block_desc = struct.Struct("=12q6i2f")      # sr_residual_norm_desc
 
@@ -925,12 +926,13 @@ class _TensorDesc(C.Structure):
 
 
 def _types():
-    global _torch, _torch_types, _current_stream
+    global _torch, _torch_types, _current_stream, _count_change
     if _torch_types is None:
         import torch
         _torch = torch
         # the handle itself where torch gives it: current_stream builds an object for it, a microsecond of a small call
         _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda i: torch.cuda.current_stream(i).cuda_stream)
+        _count_change = torch.autograd.graph.increment_version
         _torch_types = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
     return _torch_types
 
@@ -946,6 +948,11 @@ def _on(stream, device):
     """torch's current stream made `stream` (a hipStream_t): what the call allocates then belongs to the stream it runs on."""
     _types()
     return _torch.cuda.stream(_torch.cuda.ExternalStream(int(stream), device=device))
+
+
+def _written(given):
+    """Tensors of the caller's that a call wrote: torch then refuses a backward pass that wanted what they held."""
+    _count_change([t for t in given if t is not None])
 
 
 def _no_graph(what):
@@ -980,8 +987,6 @@ def _pitch(t, what, shape, dtype, dev):
 
 
 def _vector(t, what, C_, dev):
-    if t is None:
-        return None
     if t.requires_grad:
         _no_graph(what)
     if t.dtype is not _torch.float32 or t.get_device() != dev or t.dim() != 1 or t.numel() != C_ or not t.is_contiguous():
@@ -1047,6 +1052,7 @@ def residual_norm(x, y=None, gate=None, post_gain=None, post_bias=None, pre_gain
     C_ = shape[-1]
     bt = y.dtype if y is not None else branch_dtype or x.dtype
     rpg, ldg, ldy, ldh, ldn = 1, 0, 0, 0, 0
+    given = None if h is None and n is None else (h, n)
     ldx = _pitch(x, "x", shape, x.dtype, dev)
     if y is not None:
         ldy = _pitch(y, "y", shape, bt, dev)
@@ -1070,12 +1076,16 @@ def residual_norm(x, y=None, gate=None, post_gain=None, post_bias=None, pre_gain
     d = _pack_block(rows, rpg, ldx, ldy, ldg, ldh, ldn, 0, 0, 0, 0, 0, C_, st, _type_of(bt, "y"), _KINDS[kind], mask, _GATES[gate_act],
                     scale, eps)
     rc = lib().sr_op_residual_norm(dev, d, x.data_ptr(), None if y is None else y.data_ptr(), None if gate is None else gate.data_ptr(),
-                                   _vector(post_gain, "post_gain", C_, dev), _vector(post_bias, "post_bias", C_, dev),
-                                   _vector(pre_gain, "pre_gain", C_, dev), _vector(pre_bias, "pre_bias", C_, dev),
+                                   post_gain if post_gain is None else _vector(post_gain, "post_gain", C_, dev),
+                                   post_bias if post_bias is None else _vector(post_bias, "post_bias", C_, dev),
+                                   pre_gain if pre_gain is None else _vector(pre_gain, "pre_gain", C_, dev),
+                                   pre_bias if pre_bias is None else _vector(pre_bias, "pre_bias", C_, dev),
                                    None if h is None else h.data_ptr(), None if n is None else n.data_ptr(),
                                    _current_stream(dev))
     if rc:
         _check(rc)
+    if given:
+        _written(given)
     return (x if y is None else h), n
 
 
@@ -1118,6 +1128,7 @@ def residual_norm_bwd(h, y=None, dh=None, dn=None, gate=None, post_gain=None, po
     if dn is not None:
         lddn = _pitch(dn, "dn", shape, bt, dev)
     lddx = lddy = C_
+    given = None if dx is None and dy is None else (dx, dy)
     if dx is None:
         dx = _empty(h, shape, ldh)
     else:
@@ -1147,13 +1158,16 @@ def residual_norm_bwd(h, y=None, dh=None, dn=None, gate=None, post_gain=None, po
     out = [_vector_like(post_gain, C_, h) if post else None, _vector_like(post_gain, C_, h) if post and bias_grads else None,
            _vector_like(pre_gain, C_, h) if pre else None, _vector_like(pre_gain, C_, h) if pre and bias_grads else None]
     rc = lib().sr_op_residual_norm_bwd(dev, d, h.data_ptr(), None if y is None else y.data_ptr(), None if gate is None else gate.data_ptr(),
-                                       _vector(post_gain, "post_gain", C_, dev), _vector(post_bias, "post_bias", C_, dev),
-                                       _vector(pre_gain, "pre_gain", C_, dev), None if dh is None else dh.data_ptr(),
+                                       post_gain if post_gain is None else _vector(post_gain, "post_gain", C_, dev),
+                                       post_bias if post_bias is None else _vector(post_bias, "post_bias", C_, dev),
+                                       pre_gain if pre_gain is None else _vector(pre_gain, "pre_gain", C_, dev), None if dh is None else dh.data_ptr(),
                                        None if dn is None else dn.data_ptr(), dx.data_ptr(), None if dy is None else dy.data_ptr(),
                                        None if dgate is None else dgate.data_ptr(), *[None if v is None else v.data_ptr() for v in out],
                                        None if ws is None else ws.data_ptr(), need, _current_stream(dev))
     if rc:
         _check(rc)
+    if given:
+        _written(given)
     return ResidualNormGrads(dx, dy, dgate, *out)
 
 
@@ -1178,6 +1192,8 @@ class TensorList:
             if not _dense(t):
                 raise ValueError(f"tensor {i} of shape {tuple(t.shape)} and strides {tuple(t.stride())} has gaps or repeats elements")
             desc[i].data, desc[i].count, desc[i].type = t.data_ptr() or None, t.numel(), _type_of(t.dtype, f"tensor {i}")
+        # what shares a count of in-place changes: views and what they are views of.  A list made for one call does not look for them
+        self._counts = self.tensors if not upload else list({id(t): t for t in [t if t._base is None else t._base for t in self.tensors]}.values())
         # a tensor that is given other memory (t.data = ...) leaves this behind
         self._storages = [t.untyped_storage() for t in self.tensors] if upload else None
         self._h = _vp()
@@ -1253,6 +1269,7 @@ def clip_grads(grads, max_norm, scale=1.0, out=None, stream=None):
     ws = _torch.empty(grads.workspace_bytes, dtype=_torch.uint8, device=dev)
     _check(lib().sr_op_clip_grads(grads._h, out._h if out is not None else None, max_norm, scale, norm.data_ptr(), ws.data_ptr(),
                                   grads.workspace_bytes, _current_stream(grads.index)))
+    _count_change((grads if out is None else out)._counts)
     return norm
 
 

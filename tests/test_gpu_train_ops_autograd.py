@@ -63,3 +63,41 @@ def test_as_a_function_of_autograd(sh):
     for k, name in (("x", "dx"), ("y", "dy"), ("gate", "dgate"), ("post_gain", "post_gain"), ("pre_gain", "pre_gain")):
         ref, mag = want[name]
         within(leaf[k].grad.reshape(ref.shape), ref, mag, 320, name)
+
+
+def test_what_a_call_writes_counts_as_changed(sh):
+    """A backward pass that wanted the old contents is refused, as after any in-place operation, and not computed from the new ones."""
+    C = 48
+    c = case(3, (9,), C, F32, F32)
+    w = torch.ones(9, C, device="cuda", requires_grad=True)
+    mine = lambda k: c[k].clone()
+    calls = {
+        "h": lambda t: sh.residual_norm(t, mine("y"), h=t), "n": lambda t: sh.residual_norm(mine("x"), t, n=t),
+        "dx": lambda t: sh.residual_norm_bwd(mine("x"), mine("y"), t, mine("dn"), dx=t), "dy": lambda t: sh.residual_norm_bwd(mine("x"), mine("y"), mine("dh"), t, dy=t),
+        "a view": lambda t: sh.residual_norm(t[2:5], mine("y")[2:5], h=t[2:5]),
+        "clipped": lambda t: sh.clip_grads([t], 1e-3), "a clipped view": lambda t: sh.clip_grads([t[2:5]], 1e-3),
+        "a list's": lambda t: sh.clip_grads(sh.TensorList([mine("y"), t]), 1e-3), "a list's view": lambda t: sh.clip_grads(sh.TensorList([t[0], t[4]]), 1e-3),
+        "out": lambda t: sh.clip_grads([mine("x")], 1e-3, out=[t]), "a list's out": lambda t: sh.clip_grads([mine("x")], 1e-3, out=sh.TensorList([t])),
+    }
+    for name, call in calls.items():
+        t = mine("x")
+        lost = (w * t).sum()
+        with torch.no_grad():
+            call(t)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            lost.backward()
+            print(name)
+    for call in (lambda t: sh.residual_norm(t, mine("y")), lambda t: sh.residual_norm(mine("x"), t), lambda t: sh.grad_norm([t]),
+                 lambda t: sh.clip_grads([t], 1e-3, out=[mine("x")]), lambda t: sh.residual_norm_bwd(mine("x"), mine("y"), t, mine("dn"))):
+        t = mine("x")                            # only read: the backward pass goes ahead
+        kept = (w * t).sum()
+        call(t)
+        kept.backward()
+        assert torch.equal(w.grad, t)
+        w.grad = None
+    with torch.inference_mode():                 # tensors without a count
+        t = torch.ones(9, C, device="cuda")
+    sh.residual_norm(t, mine("y"), h=t)
+    sh.clip_grads([t], 1e-3)
+    with torch.inference_mode():
+        sh.clip_grads(sh.TensorList([t, t[:0]]), 1e-3)
