@@ -469,8 +469,9 @@ int sr_tensors_workspace(const sr_tensors* t, size_t* bytes);
 int sr_op_grad_norm(const sr_tensors* grads, float scale, float* d_norm, float* d_norms, void* workspace, size_t workspace_bytes,
                     void* hip_stream);
 /* Gradient clipping as Keras 2.2.4's `clipnorm` does it (optimizers.py get_gradients / clip_norm): with norm as above, every element
- * becomes g * scale * (max_norm / norm if norm > max_norm, else 1), rounded once to its type.  A NaN norm clips nothing, an
- * infinite one leaves zeros (NaN where the infinity was), as the formula says; d_norm tells.  `out` (NULL: in place): a list
+ * becomes g * scale * (max_norm / norm if norm > max_norm, else 1), in fp32 and then rounded to its type.  A NaN norm clips nothing, an
+ * infinite one leaves zeros (NaN where the infinity was), as the formula says; d_norm tells.  Finite gradients whose norm only fp32 does
+ * not hold (d_norm shows an infinity) are clipped by that norm all the same.  `out` (NULL: in place): a list
  * of the same counts and types that is written instead; each of its tensors is the gradient itself or overlaps none. */
 int sr_op_clip_grads(const sr_tensors* grads, const sr_tensors* out, float max_norm, float scale, float* d_norm, void* workspace,
                      size_t workspace_bytes, void* hip_stream);

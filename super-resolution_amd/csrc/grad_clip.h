@@ -33,9 +33,18 @@ struct ClipArgs {
     float* norm;                    // written by workgroup 0
 };
 
-// All 256 threads of a workgroup: the factor that brings the gradients' norm down to max_norm, 1 where it is not above it (or NaN).
-// Every workgroup adds the partial sums in the same order, so all have the same bits.
-__device__ __forceinline__ float clip_factor(const ClipArgs& c, double* lds4) {
+// What a gradient is multiplied by: f, then 2^e.  e is 0 but where the product is below fp32's normal range (gradients near its upper
+// end and a small bound, for instance: 1e6 elements of 1e38 and a bound of 1), which one fp32 factor would hold with a few bits or not
+// at all; f is then in [0.5, 1).
+struct GradScale {
+    float f;
+    int e;
+    __device__ __forceinline__ float operator()(float g) const { return ldexpf(g * f, e); }
+};
+
+// All 256 threads of a workgroup: `scale` times the factor that brings the gradients' norm down to max_norm, 1 where it is not above it
+// (or NaN).  Every workgroup adds the partial sums in the same order, so all have the same bits.
+__device__ __forceinline__ GradScale clip_factor(const ClipArgs& c, float scale, double* lds4) {
     double s = 0.0;
     const double q0 = (double)c.s0 * c.s0, q1 = (double)c.s1 * c.s1;
 #pragma unroll 8
@@ -45,7 +54,15 @@ __device__ __forceinline__ float clip_factor(const ClipArgs& c, double* lds4) {
     __syncthreads();
     const double norm = sqrt((lds4[0] + lds4[1]) + (lds4[2] + lds4[3]));
     if (blockIdx.x == 0 && threadIdx.x == 0 && c.norm) *c.norm = (float)norm;
-    return norm > (double)c.max_norm ? (float)((double)c.max_norm / norm) : 1.f;
+    const double factor = norm > (double)c.max_norm ? (double)c.max_norm / norm : 1.0;
+    constexpr float least = 1.17549435e-38f;
+    const float f = (float)factor * scale;
+    if ((float)factor >= least && fabsf(f) >= least) return {f, 0};
+    const double p = factor * (double)scale;      // the factor alone may be out of range where the product is not
+    if (p == 0.0 || fabs(p) >= (double)least) return {(float)p, 0};
+    int e;
+    const double m = frexp(p, &e);
+    return {(float)m, e};
 }
 
 }  // namespace sr

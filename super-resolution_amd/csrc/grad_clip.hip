@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(256) grad_norm_kernel(const TABLE_T t, const d
 }
 
 template <bool NT, typename T>
-__device__ __forceinline__ void scale_run(const T* src, T* dst, uint32_t n, float f) {
+__device__ __forceinline__ void scale_run(const T* src, T* dst, uint32_t n, GradScale f) {
     constexpr int V = 16 / sizeof(T);
     const uint32_t nv = n / V;
 #pragma unroll 4
@@ -160,20 +160,20 @@ __device__ __forceinline__ void scale_run(const T* src, T* dst, uint32_t n, floa
         float v[V];
         load_vec<T, V>(src + (size_t)i * V, v);
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] *= f;
+        for (int k = 0; k < V; ++k) v[k] = f(v[k]);
         if (NT) store_vec_nt<T, V>(dst + (size_t)i * V, v);
         else store_vec<T, V>(dst + (size_t)i * V, v);
     }
     const uint32_t t = nv * V + threadIdx.x;
-    if (t < n) dst[t] = (T)((float)src[t] * f);
+    if (t < n) dst[t] = (T)f((float)src[t]);
 }
 
 template <bool NT, typename TABLE_T>
 __global__ void __launch_bounds__(256) grad_scale_kernel(const TABLE_T t, const ClipArgs a) {
     __shared__ double lds4[4];
     const Chunk c = chunk_of(t, blockIdx.x);
-    const float f = clip_factor(a, lds4) * a.s0;
-    if (f == 1.f && c.src == c.dst) return;   // in place and nothing to do
+    const GradScale f = clip_factor(a, a.s0, lds4);
+    if (f.f == 1.f && f.e == 0 && c.src == c.dst) return;   // in place and nothing to do
     if (c.type == SR_T_F32) scale_run<NT>((const float*)c.src, (float*)c.dst, c.n, f);
     else if (c.type == SR_T_BF16) scale_run<NT>((const bf16_t*)c.src, (bf16_t*)c.dst, c.n, f);
     else scale_run<NT>((const f16_t*)c.src, (f16_t*)c.dst, c.n, f);

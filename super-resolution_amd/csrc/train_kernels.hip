@@ -1039,8 +1039,7 @@ hipError_t launch_mse_grad(const float* pred, const float* target, float* g, dou
 
 // ================================================================== Adam (Keras 2.2.4 optimizers.py) and re-pack
 __device__ __forceinline__ void adam_update(float* __restrict__ p, float* __restrict__ m, float* __restrict__ v,
-                                            const float* __restrict__ g, long i, float lr_t, float b1, float b2, float eps, float gscale) {
-    const float gi = g[i] * gscale;
+                                            float gi, long i, float lr_t, float b1, float b2, float eps) {
     const float mi = b1 * m[i] + (1.f - b1) * gi;
     const float vi = b2 * v[i] + (1.f - b2) * gi * gi;
     m[i] = mi;
@@ -1052,7 +1051,7 @@ __global__ void adam_kernel(float* __restrict__ p, float* __restrict__ m, float*
                             long n, float lr_t, float b1, float b2, float eps, float gscale) {
     const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= n) return;
-    adam_update(p, m, v, g, i, lr_t, b1, b2, eps, gscale);
+    adam_update(p, m, v, g[i] * gscale, i, lr_t, b1, b2, eps);
 }
 
 // Keras 2.2.4 `clipnorm` (optimizers.py get_gradients: all gradients scaled by clipnorm / norm where their global norm reaches
@@ -1063,8 +1062,8 @@ __global__ void __launch_bounds__(256) adam_clip_kernel(float* __restrict__ p, f
                                                         const float* __restrict__ g, long n, float lr_t, float b1, float b2, float eps,
                                                         float gscale, const ClipArgs c) {
     __shared__ double lds4[4];
-    const float gs = gscale * clip_factor(c, lds4);
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) adam_update(p, m, v, g, i, lr_t, b1, b2, eps, gs);
+    const GradScale gs = clip_factor(c, gscale, lds4);
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) adam_update(p, m, v, gs(g[i]), i, lr_t, b1, b2, eps);
 }
 
 hipError_t launch_adam_clip(float* p, float* m, float* v, const float* g, long n, float lr_t, float b1, float b2, float eps,
