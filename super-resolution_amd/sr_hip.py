@@ -1181,17 +1181,14 @@ class TensorList:
     def __init__(self, tensors, upload=True):
         self.tensors = list(tensors)
         _types()
-        self.device = self.tensors[0].device if self.tensors else _torch.device("cuda", _torch.cuda.current_device())
-        if self.device.type != "cuda":
-            raise ValueError(f"tensor 0 is on {self.device}: these operators have no CPU fallback")
-        self.index = self.device.index
-        desc = (_TensorDesc * max(len(self.tensors), 1))()
-        for i, t in enumerate(self.tensors):
-            if t.device != self.device:
-                raise ValueError(f"tensor {i} is on {t.device}, tensor 0 on {self.device}")
-            if not _dense(t):
-                raise ValueError(f"tensor {i} of shape {tuple(t.shape)} and strides {tuple(t.stride())} has gaps or repeats elements")
-            desc[i].data, desc[i].count, desc[i].type = t.data_ptr() or None, t.numel(), _type_of(t.dtype, f"tensor {i}")
+        try:
+            desc = self._describe()
+        except AttributeError:
+            for i, t in enumerate(self.tensors):
+                if not isinstance(t, _torch.Tensor):
+                    more = ": leave out what has no gradient" if t is None else ""
+                    raise ValueError(f"tensor {i} is not a tensor but {type(t).__name__}{more}") from None
+            raise
         # what shares a count of in-place changes: views and what they are views of.  A list made for one call does not look for them
         self._counts = self.tensors if not upload else list({id(t): t for t in [t if t._base is None else t._base for t in self.tensors]}.values())
         # a tensor that is given other memory (t.data = ...) leaves this behind
@@ -1203,6 +1200,20 @@ class TensorList:
         self.workspace_bytes = need.value
         if upload and not _torch.cuda.is_current_stream_capturing():
             _check(lib().sr_tensors_upload(self._h))
+
+    def _describe(self):
+        self.device = self.tensors[0].device if self.tensors else _torch.device("cuda", _torch.cuda.current_device())
+        if self.device.type != "cuda":
+            raise ValueError(f"tensor 0 is on {self.device}: these operators have no CPU fallback")
+        self.index = self.device.index
+        desc = (_TensorDesc * max(len(self.tensors), 1))()
+        for i, t in enumerate(self.tensors):
+            if t.device != self.device:
+                raise ValueError(f"tensor {i} is on {t.device}, tensor 0 on {self.device}")
+            if not _dense(t):
+                raise ValueError(f"tensor {i} of shape {tuple(t.shape)} and strides {tuple(t.stride())} has gaps or repeats elements")
+            desc[i].data, desc[i].count, desc[i].type = t.data_ptr() or None, t.numel(), _type_of(t.dtype, f"tensor {i}")
+        return desc
 
     def __len__(self):
         return len(self.tensors)
