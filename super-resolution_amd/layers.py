@@ -308,8 +308,8 @@ class Adam(object):
         self.lr, self.beta_1, self.beta_2 = float(lr), float(beta_1), float(beta_2)
         self.epsilon = 1e-7 if epsilon is None else float(epsilon)      # K.epsilon()
         self.clipnorm = float(clipnorm or 0.)
-        if not 0. <= self.clipnorm < 3e38:
-            raise ValueError('clipnorm must be 0 (no clipping) or positive and finite, got %r' % (clipnorm,))
+        if not 0. <= self.clipnorm < 3e38 or (self.clipnorm and not np.float32(self.clipnorm)):     # below float32 it would be 0: off
+            raise ValueError('clipnorm must be 0 (no clipping) or a positive finite float32, got %r' % (clipnorm,))
         # optimizer.iterations: ONE counter per Adam instance, shared by every model compiled with it (the reference
         # compiles generator, discriminator and tecogan with the same instance, TecoGAN.py:111-131); the moments belong
         # to each model's own train function

@@ -162,6 +162,12 @@ def _check(rc, ctx=None):
     raise RuntimeError(msg)
 
 
+def _clipnorm(v):
+    if v and not C.c_float(v).value:
+        raise ValueError(f"clipnorm {v!r} is below float32, where it would mean no clipping")
+    return v
+
+
 def _f32(a):
     return np.ascontiguousarray(a, dtype=np.float32)
 
@@ -398,7 +404,7 @@ class Context:
     def set_clipnorm(self, clipnorm):
         """Global gradient norm that every later optimizer step of this context clips to; 0: off (include/sr_hip.h
         sr_train_set_clipnorm)."""
-        _check(lib().sr_train_set_clipnorm(self._h, clipnorm), self._h)
+        _check(lib().sr_train_set_clipnorm(self._h, _clipnorm(clipnorm)), self._h)
 
     def grad_norm(self):
         """The gradient norm, before clipping, of the last step with clipping."""
@@ -584,7 +590,7 @@ class Discriminator:
 
     def set_clipnorm(self, clipnorm):
         """As Context.set_clipnorm, for the discriminator's own steps (apply and those of tecogan_iteration)."""
-        self._check(lib().sr_disc_set_clipnorm(self._h, clipnorm))
+        self._check(lib().sr_disc_set_clipnorm(self._h, _clipnorm(clipnorm)))
 
     def grad_norm(self):
         """The gradient norm, before clipping, of the last such step with clipping."""

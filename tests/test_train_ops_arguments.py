@@ -16,3 +16,15 @@ def test_lists_hold_tensors_only(bad):
     if bad is None:
         with pytest.raises(ValueError, match="leave out what has no gradient"):
             sr_hip.grad_norm([None])
+
+
+def test_a_bound_below_float32_is_not_taken_for_no_bound():
+    from layers import Adam
+    with pytest.raises(ValueError, match="clipnorm"):
+        Adam(clipnorm=1e-46)
+    assert Adam(clipnorm=1e-45).clipnorm == 1e-45 and Adam(clipnorm=0.0).clipnorm == 0.0
+    for cls in (sr_hip.Context, sr_hip.Discriminator):
+        c = object.__new__(cls)
+        c._h = None
+        with pytest.raises(ValueError, match="below float32"):
+            c.set_clipnorm(1e-46)
