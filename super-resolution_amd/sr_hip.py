@@ -1073,7 +1073,7 @@ def residual_norm(x, y=None, gate=None, post_gain=None, post_bias=None, pre_gain
         raise ValueError("without y there is only norms='pre', and neither gate nor h")
     if mask & 2:
         if n is None:
-            n = _empty(y, shape, ldy) if y is not None else _torch.empty(shape, dtype=bt, device=x.device)
+            n = _empty(y, shape, ldy if y.shape == shape else 0) if y is not None else _torch.empty(shape, dtype=bt, device=x.device)
             ldn = C_
         else:
             ldn = _pitch(n, "n", shape, bt, dev)
@@ -1141,7 +1141,7 @@ def residual_norm_bwd(h, y=None, dh=None, dn=None, gate=None, post_gain=None, po
         lddx = _pitch(dx, "dx", shape, h.dtype, dev)
     if branch:
         if dy is None:
-            dy = _empty(like, shape, ldy if y is not None else lddn)
+            dy = _empty(y, y.shape, ldy) if y is not None else dn.new_empty(shape)
         else:
             lddy = _pitch(dy, "dy", shape, bt, dev)
     elif dy is not None:

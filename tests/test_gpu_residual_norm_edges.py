@@ -108,3 +108,22 @@ def test_gradient_of_far_gates(sh, monkeypatch, C, lead, gate):
                 if v is not None:
                     ref, mag = want[name]
                     within(v.reshape(ref.shape), ref, mag, K, name)
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_shapes_of_outputs(sh, strided):
+    """Tensors that hold the stream's rows in other leading dimensions: h and n come in the stream's shape, dy in y's."""
+    C = 40
+    c = case(5, (12,), C, F32, BF16)
+    wide = {k: torch.zeros(12, 3 * C, device="cuda", dtype=c[k].dtype) for k in ("x", "y", "dh", "dn")}
+    v = {}
+    for k, w in wide.items():
+        w[:, :C].copy_(c[k])
+        v[k] = (w[:, :C] if strided else c[k]).unflatten(0, (12,) if k in ("y", "dn") else (3, 4))
+    h, n = sh.residual_norm(v["x"], v["y"])
+    flat = sh.residual_norm(c["x"], c["y"])
+    assert h.shape == n.shape == (3, 4, C) and torch.equal(h.view(12, C), flat[0]) and torch.equal(n.view(12, C), flat[1])
+    g = sh.residual_norm_bwd(h, v["y"], v["dh"], v["dn"])
+    assert g.dx.shape == (3, 4, C) and g.dy.shape == (12, C)
+    g = sh.residual_norm_bwd(h, None, v["dh"], v["dn"], norms="pre", branch=True)
+    assert g.dx.shape == g.dy.shape == (3, 4, C) and g.dy.dtype == BF16
