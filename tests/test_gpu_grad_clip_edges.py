@@ -79,3 +79,26 @@ def test_clipped_step_is_the_step_of_clipped_gradients(sh, weights7, size, max_n
         assert (x == y).all(), n
         moved += int((x != weights7[n]).sum())
     assert moved > 0
+
+
+@pytest.mark.parametrize("n", [900, 901, 2000])
+def test_norm_of_each_of_many_tensors_without_records(sh, n):
+    """Lists made for one call and captured ones: the tensors' partial sums travel in the kernel arguments, 900 tensors a launch."""
+    ts = [uniform(i, 1 + i * 7 % 50, -1.0, 1.0) for i in range(n)]
+    norm, each = sh.grad_norm(sh.TensorList(ts), per_tensor=True)
+    got = sh.grad_norm(ts, per_tensor=True)
+    assert torch.equal(got[0], norm) and torch.equal(got[1], each)
+    want = torch.stack([(t.double() ** 2).sum().sqrt() for t in ts])
+    assert float(((each.double() - want).abs() - want * (U + 1e-12)).max()) <= 0
+    lst = sh.TensorList(ts)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = sh.grad_norm(lst, per_tensor=True)
+    for i in range(3):
+        for t in ts:
+            t.mul_(0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = sh.grad_norm(ts, per_tensor=True)
+        assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1]) and torch.equal(eager[1], each * 0.5 ** (i + 1))
