@@ -81,7 +81,7 @@ struct Team {
     static constexpr bool BLK = BLK_, TAIL = TAIL_;
     int lanes, lane, row, rows;      // lanes of a team, this thread's lane, its team's number in the workgroup, teams in the workgroup
     int tl, C, part;
-    float* red;                      // BLK: [2][16][E] floats
+    float* red;                      // BLK: [2][16][8] floats: two buffers, up to 8 sums of up to 16 waves
     int phase = 0;
 
     __device__ Team(int tl_, int C_, float* red_) : tl(tl_), C(C_), part(C_ % VEC), red(red_) {
@@ -108,6 +108,7 @@ struct Team {
     // sums of K values over the team, in every lane
     template <int K>
     __device__ __forceinline__ void sum(float (&v)[K]) {
+        static_assert(K <= 8, "places of a wave in red");
 #pragma unroll
         for (int k = 0; k < K; ++k) v[k] = lanes_sum(v[k], BLK ? 6 : tl);
         if (BLK) {
@@ -457,7 +458,7 @@ constexpr int bwd_sums() { return (FULL ? 4 : GATE == G_SHARED ? 3 : 2) + (GATE 
 //   A = sum T hat(y) (or T y), B = sum T   (T with the scale):  dpost_gain = a A, dpost_bias = a B, dgate = a' (post_gain A + post_bias B)
 template <typename TS, typename TB, int E, int VEC, bool BLK, bool TAIL, int GATE, bool FULL>
 __global__ void __launch_bounds__(BLK ? 1024 : 512, BLK ? 4 : 3) rn_bwd_kernel(const BwdArgs a) {
-    extern __shared__ float lds[];   // the sums, then BLK's [2][16][E] floats
+    extern __shared__ float lds[];   // the sums, then BLK's [2][16][8] floats
     constexpr bool ROW = GATE == G_ROW || GATE == G_GROUP;
     constexpr int NS = bwd_sums<GATE, FULL, BLK>();
     enum { S_PW, S_QW, S_PB, S_QB, S_GATE = NS - 1 };
@@ -753,7 +754,7 @@ __global__ void __launch_bounds__(1024) rn_join_kernel(const JoinArgs a) {
 // ------------------------------------------------------------------------------------------------- host
 struct Shape {
     bool blk;
-    int e, vec;                      // elements of a lane, of a vector
+    int e;                           // elements of a lane
     int threads, tl, teams;          // threads of a workgroup, log2 of a team's lanes (rows within a wave), teams of a workgroup
 };
 
@@ -761,7 +762,6 @@ Shape shape_of(const sr_residual_norm_desc* d, int e) {
     Shape s;
     const int lanes = (d->channels + e - 1) / e;
     s.e = e;
-    s.vec = d->stream_type == SR_T_F32 ? 4 : e;
     s.blk = d->channels > WAVE_C;
     s.tl = 0;
     while (!s.blk && (1 << s.tl) < lanes) ++s.tl;
