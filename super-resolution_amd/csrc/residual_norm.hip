@@ -15,8 +15,8 @@
 // once: a group of lanes (a "team") holds it in registers across all sums of the row, and the backward pass takes the row
 // statistics again from what it holds instead of reading them.  Rows of up to 512 channels belong to 1..64 lanes of a wave, several
 // rows to a wave, and their sums are lane exchanges; longer rows belong to a workgroup, which joins its waves' sums in LDS.  A lane
-// holds 8 elements of a row (4 in the backward pass of long rows where 8 need more registers than there are) and has the same places of
-// the team's next row on their way.  All sums and the values between them are fp32; tensors of 16 bits are rounded
+// holds 8 elements of a row (4 in the backward pass of 513 to 4096 channels where 8 need more registers than there are; above that it is
+// 8 with what it spills, see bwd_plan) and has the same places of the team's next row on their way.  All sums and the values between them are fp32; tensors of 16 bits are rounded
 // once, when they are stored.
 #include "op_host.h"
 #include "row_math.h"
@@ -867,6 +867,12 @@ BwdPlan bwd_plan(const sr_residual_norm_desc* d, bool gate, unsigned rpg, bool f
     //   16 bits, gated, % 8:   640: 54.6 / 51.0; 1304: 51 / 59; 2312: 50 / 61; 3400: 49 / 53;   other channels: 1541: 64 / 59; 4095: 68 / 57
     //   fp32, no gate, % 4, where 4 elements make rows of 9 to 12 waves, of which a CU holds one: 2056: 53 / 68, layer 63 / 75; 2600:
     //   55 / 62, 66 / 69;   else: 776: 59.9 / 56.3, 76 / 60; 1544: 57.6 / 53.7; 3400: 57 / 59, 69 / 67;   other channels: 2050: 66 / 54
+    // Above 4096 channels 1024 lanes of 4 do not hold a row: 8 in any case, and most of these kernels spill.  Bytes of scratch a lane, gains
+    // only / all sums: fp32 streams 0 / 0..20 and gated 0..68 / 44..108 where C % 4 == 0, else 108..148 / 236..268 and gated 200..280 /
+    // 316..380; 16 bits gated 0 / 20..28 where C % 8 == 0, else 0 / 52 and gated 60..116 / 124..188.  us at 12 M elements, 5120 and 6145
+    // channels: bf16 36 / 44 and 37 / 52, gated 49 / 59 and 56 / 79; fp32 58 / 67 and 73 / 93, gated 95 / 104 and 109 / 127 (the traffic alone: 27,
+    // gated 36; 53, gated 71).  Of the shorter rows these do: 16 bits, odd, no gate, all sums (52); fp32 streams of odd channels with a gate
+    // (12..44 above 512 channels, 28..60 for fp32 branches below).
     const int wide = (C + 255) / 256;
     const bool e8 = d->stream_type == SR_T_F32 ? !gate && whole4 && wide > 8 && wide <= 12 : !gate || (whole8 && C > 1024);
     q.s = shape_of(d, C <= WAVE_C || C > 4096 || e8 ? 8 : 4);
